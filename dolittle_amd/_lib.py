@@ -131,6 +131,11 @@ class TensorInfo(C.Structure):
                 ("dtype", C.c_int32)]
 
 
+class BatchShape(C.Structure):
+    _fields_ = [("batch", C.c_uint64), ("rows", C.c_uint64), ("query_heads", C.c_uint64), ("kv_heads", C.c_uint64),
+                ("width", C.c_uint64), ("capacity", C.c_uint64)]
+
+
 # name -> argument types (all return int status)
 SIGNATURES = {
     "dl_device_open": [cint, vpp],
@@ -168,6 +173,13 @@ SIGNATURES = {
     "dl_projection_packed_bytes": [u64, u64, u64p],
     "dl_projection_pack": [vp, vp, vp, u64, u64],
     "dl_projection_packed": [vp, vp, vp, vp, u64, u64, u64, vp],
+    "dl_attention_shared_bytes": [C.POINTER(BatchShape), u64, u64p],
+    "dl_attention_shared": [vp, cint, C.POINTER(BatchShape), vp, vp, vp, u64, vp, vp, vp, vp, vp, vp, u64],
+    "dl_attention_weighted_bytes": [C.POINTER(BatchShape), u64, u64p],
+    "dl_attention_weighted": [vp, cint, C.POINTER(BatchShape), vp, vp, vp, u64, vp, vp, vp, vp, vp, vp, vp, vp, u64],
+    "dl_cache_append": [vp, cint, C.POINTER(BatchShape), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_double],
+    "dl_cache_evict_bytes": [C.POINTER(BatchShape), u64, u64p],
+    "dl_cache_evict": [vp, cint, C.POINTER(BatchShape), vp, vp, vp, vp, vp, vp, vp, vp, u64, u64, u64, vp, u64],
     "dl_qwen3_create": [vp, vp, C.POINTER(Qwen3Config), vpp],
     "dl_qwen3_destroy": [vp],
     "dl_qwen3_fill_synthetic": [vp, vp, u64, C.c_float],

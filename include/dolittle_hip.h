@@ -201,6 +201,85 @@ int dl_prefill_attention(dl_queue* queue, const void* q_rot, const void* k_cache
 int dl_prefill_gate_up(dl_queue* queue, const void* input, const void* packed, void* output,
                        void* workspace, uint64_t rows, uint64_t hidden, uint64_t ffn);
 
+/* ------------------------------- a batch over a shared prefix and own caches */
+/* Attention and cache operations of a batch of sequences.  No reference
+ * counterpart: the reference decodes one sequence over one contiguous cache
+ * (src/inference/cache/contiguous.cpp).  Tolerance, not bit-exact: matrix-core
+ * accumulation and FP32 exponentials; dl_attention is the conforming operation.
+ *
+ * Operands are dense device arrays, in the catalog's row layout:
+ *   query, output    [batch][rows][query_heads][width]
+ *   prefix K and V   [prefix][kv_heads][width], the same for every sequence
+ *   own K and V      [batch][capacity][kv_heads][width]
+ *   lengths          uint64 [batch]: rows of each own cache in use (a length
+ *                    above the capacity counts as the capacity)
+ *   slots            uint32 [batch][kv_heads][capacity]: the position of the
+ *                    row that each slot holds
+ *   weights          FP32 [batch][kv_heads][capacity]: the attention that each
+ *                    slot's row received
+ * dtype is DL_BF16 or DL_F32.  Any element-aligned address and any width are
+ * accepted; 16-byte aligned addresses and head rows run fastest.  What lies past a length is neither used nor
+ * written.  No operation allocates, waits, or uses atomics on results: the
+ * same call gives the same bits, and calls may be captured into graphs.  A
+ * workspace belongs to one call at a time; its contents need not survive. */
+typedef struct dl_batch_shape {
+  uint64_t batch;       /* sequences */
+  uint64_t rows;        /* new rows per sequence: 1 for a decode step */
+  uint64_t query_heads; /* a multiple of kv_heads */
+  uint64_t kv_heads;
+  uint64_t width;       /* features of a head */
+  uint64_t capacity;    /* slots of each own cache, at least 1 */
+} dl_batch_shape;
+
+/* out = softmax(scale * Q K^T) V over the prefix and the sequence's own cache,
+ * the prefix read once for the whole batch.  `lengths` includes the new rows,
+ * which are the last `rows` of each cache: row i sees the prefix and own slots
+ * j < length - rows + i + 1.  A row that sees no key is zeros; a key that a
+ * row does not see has no effect on it, infinities and NaN included.  Widths
+ * up to 256.  The prefix may be empty (its pointers null).  `scale` is a
+ * device word, as dl_attention's. */
+int dl_attention_shared_bytes(const dl_batch_shape* shape, uint64_t prefix, uint64_t* bytes);
+int dl_attention_shared(dl_queue* queue, int dtype, const dl_batch_shape* shape, const void* query,
+                        const void* prefix_key, const void* prefix_value, uint64_t prefix, const void* key,
+                        const void* value, const uint64_t* lengths, void* output, const float* scale, void* workspace,
+                        uint64_t workspace_bytes);
+/* dl_attention_shared, and for every own slot j < length
+ *   weights_out[b][h][j] = weights[b][h][j] + sum of the slot's softmax weights
+ * over the new rows and the query heads of KV head h.  weights_out may be
+ * weights. */
+int dl_attention_weighted_bytes(const dl_batch_shape* shape, uint64_t prefix, uint64_t* bytes);
+int dl_attention_weighted(dl_queue* queue, int dtype, const dl_batch_shape* shape, const void* query,
+                          const void* prefix_key, const void* prefix_value, uint64_t prefix, const void* key,
+                          const void* value, const uint64_t* lengths, const float* weights, float* weights_out,
+                          void* output, const float* scale, void* workspace, uint64_t workspace_bytes);
+/* Appends `rows` rows per sequence: row i enters slot lengths[b] + i (lengths
+ * before the call) with K rotated at position positions[b] + i, V copied,
+ * weight 0 and its position in `slots` (its low 32 bits); query_out is the
+ * query rotated at the same positions (it may be query).  The rotation is
+ * dl_rotary's in FP32, rounded to the storage type once (dl_rotary rounds the
+ * cosine, the sine and each product; in FP32 storage the bits are the same).
+ * lengths_out and positions_out are advanced by `rows`; each may be its input.
+ * Rows past the capacity are dropped and the length stays at the capacity. */
+int dl_cache_append(dl_queue* queue, int dtype, const dl_batch_shape* shape, const void* query, const void* key,
+                    const void* value, void* query_out, void* keys, void* values, const uint64_t* lengths,
+                    uint64_t* lengths_out, const uint64_t* positions, uint64_t* positions_out, uint32_t* slots,
+                    float* weights, double theta);
+/* Cuts every sequence that holds more than `budget` rows to `budget`, per KV
+ * head: rows at a position below `sinks` or within `recent` of the head's
+ * newest position stay, then those of the largest weight (NaN as -infinity,
+ * equal weights by the lower slot).  sinks + recent must not exceed budget
+ * (head positions are distinct).  In place, moving the fewest rows: the j-th
+ * slot below the budget whose row does not stay takes the j-th row at or above
+ * it that does; attention does not depend on the order, and `slots` says which
+ * position a slot holds.  slots_out, weights_out and lengths_out may be their
+ * inputs; their entries past the new length are left as they were.  The
+ * shape's rows and query_heads are not used. */
+int dl_cache_evict_bytes(const dl_batch_shape* shape, uint64_t budget, uint64_t* bytes);
+int dl_cache_evict(dl_queue* queue, int dtype, const dl_batch_shape* shape, void* keys, void* values,
+                   const uint64_t* lengths, uint64_t* lengths_out, const uint32_t* slots, uint32_t* slots_out,
+                   const float* weights, float* weights_out, uint64_t budget, uint64_t sinks, uint64_t recent,
+                   void* workspace, uint64_t workspace_bytes);
+
 /* -------------------------------------------------------------- Qwen3 model */
 typedef struct dl_qwen3 dl_qwen3;
 
