@@ -40,9 +40,11 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr float kLog2e = 0x1.715476p+0f;
-// A maximum is raised only when a score passes it by this much: exponentials
-// stay below e^8, and most steps rescale nothing.
-constexpr float kSlack = 8.0f;
+// Scores are in units of ln 2 from the first maximum on: exponentials are the
+// hardware's exp2 of one fused multiply-add.  A maximum is raised only when a
+// score passes it by kSlack: exponentials stay below 2^12, and most steps
+// rescale nothing.
+constexpr float kSlack = 12.0f;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -51,23 +53,26 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // 16-byte aligned.
 enum class Access { kWhole, kPieces, kElements };
 
-// N consecutive elements from `at` on as 32-bit words; zeros past the width.
+// N consecutive elements `offset` bytes past a base that the wavefront shares,
+// of which the row's features from `at` on; zeros past the width.
 template <class T, int N, Access A>
-__device__ __forceinline__ void load_words(const T* row, int at, int width, uint32_t* out) {
+__device__ __forceinline__ void load_words(const char* base, uint32_t offset, int at, int width, uint32_t* out) {
   constexpr int kWords = N * sizeof(T) / 4;
+  const char* p = base + offset;
   if constexpr (A == Access::kElements) {
+    const T* e = reinterpret_cast<const T*>(p);
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
       if constexpr (sizeof(T) == 4) {
-        out[i] = at + i < width ? __float_as_uint(row[at + i]) : 0u;
+        out[i] = at + i < width ? __float_as_uint(e[i]) : 0u;
       } else {
-        const uint32_t lo = at + 2 * i < width ? row[at + 2 * i] : 0u;
-        const uint32_t hi = at + 2 * i + 1 < width ? row[at + 2 * i + 1] : 0u;
+        const uint32_t lo = at + 2 * i < width ? e[2 * i] : 0u;
+        const uint32_t hi = at + 2 * i + 1 < width ? e[2 * i + 1] : 0u;
         out[i] = lo | (hi << 16);
       }
     }
   } else if constexpr (kWords == 2) {
-    const u32x2 v = A == Access::kWhole || at < width ? *reinterpret_cast<const u32x2*>(row + at) : u32x2{};
+    const u32x2 v = A == Access::kWhole || at < width ? *reinterpret_cast<const u32x2*>(p) : u32x2{};
     out[0] = v.x;
     out[1] = v.y;
   } else {
@@ -75,7 +80,7 @@ __device__ __forceinline__ void load_words(const T* row, int at, int width, uint
 #pragma unroll
     for (int i = 0; i < kWords / 4; ++i) {
       const u32x4 v =
-          A == Access::kWhole || at + i * kPer < width ? *reinterpret_cast<const u32x4*>(row + at + i * kPer) : u32x4{};
+          A == Access::kWhole || at + i * kPer < width ? reinterpret_cast<const u32x4*>(p)[i] : u32x4{};
       out[4 * i] = v.x;
       out[4 * i + 1] = v.y;
       out[4 * i + 2] = v.z;
@@ -84,10 +89,9 @@ __device__ __forceinline__ void load_words(const T* row, int at, int width, uint
   }
 }
 
-// exp(v) by the hardware's exp2; v <= kSlack or NaN.
-__device__ __forceinline__ float fast_exp(float v) { return __builtin_amdgcn_exp2f(v * kLog2e); }
+__device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
 // The value subtracted from scores: 0 while no score is finite, so that
-// exp(-inf - m) is 0 and not NaN.
+// exp2(-inf - m) is 0 and not NaN.
 __device__ __forceinline__ float reference_of(float m) { return m == -INFINITY ? 0.0f : m; }
 
 __device__ __forceinline__ float group_max(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -109,25 +113,31 @@ struct Operands<uint16_t, D, A> {
   using T = uint16_t;
   static constexpr int kKeys = 32, kTiles = 2, kSteps = D / 32, C = D / 16;
   static constexpr int kValueRows = 8;
-  struct Keys {
-    u32x4 v[kTiles][kSteps];
-  };
   struct Values {
     uint32_t v[kValueRows][C / 2];
   };
-  // A row's features (4 s + g) 8 .. of product step s.
-  static __device__ __forceinline__ void load_row(const T* row, int g, int width, u32x4* out) {
+  // A row's features (4 s + g) 8 .. of product step s; `offset` holds the lane's own 16 g bytes.
+  static __device__ __forceinline__ void load_row(const char* base, uint32_t offset, int g, int width, u32x4* out) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) load_words<T, 8, A>(row, (4 * s + g) * 8, width, reinterpret_cast<uint32_t*>(&out[s]));
+    for (int s = 0; s < kSteps; ++s)
+      load_words<T, 8, A>(base + 64 * s, offset, (4 * s + g) * 8, width, reinterpret_cast<uint32_t*>(&out[s]));
   }
   // The key of value row r in the order in which P holds them.
   static __device__ __forceinline__ int value_key(int g, int r) { return (r / 4) * 16 + 4 * g + r % 4; }
-  static __device__ __forceinline__ void scores(const u32x4* k, const u32x4* q, f32x4& s) {
+  // Scores of NQ row tiles against NK key tiles, the chains side by side.
+  template <int NQ, int NK>
+  static __device__ __forceinline__ void scores(const u32x4 (&k)[NK][kSteps], const u32x4 (&q)[NQ][kSteps], f32x4 (&s)[NQ][NK]) {
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
-      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[i]), __builtin_bit_cast(bf16x8, q[i]), s, 0,
-                                                  0, 0);
+#pragma unroll
+      for (int t = 0; t < NQ; ++t)
+#pragma unroll
+        for (int u = 0; u < NK; ++u)
+          s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[u][i]),
+                                                            __builtin_bit_cast(bf16x8, q[t][i]),
+                                                            i ? s[t][u] : f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
   }
+  static constexpr uint32_t kSigns = 0x80008000u;
   // The first operand of feature tile j.
   static __device__ __forceinline__ bf16x8 value_tile(const Values& v, int j) {
     u32x4 w;
@@ -162,24 +172,30 @@ struct Operands<float, D, A> {
   using T = float;
   static constexpr int kKeys = 16, kTiles = 1, kSteps = D / 16, C = D / 16;
   static constexpr int kValueRows = 4;
-  struct Keys {
-    u32x4 v[kTiles][kSteps];
-  };
   struct Values {
     uint32_t v[kValueRows][C];
   };
-  static __device__ __forceinline__ void load_row(const T* row, int g, int width, u32x4* out) {
+  // `offset` holds the lane's own 16 g bytes.
+  static __device__ __forceinline__ void load_row(const char* base, uint32_t offset, int g, int width, u32x4* out) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) load_words<T, 4, A>(row, (4 * s + g) * 4, width, reinterpret_cast<uint32_t*>(&out[s]));
+    for (int s = 0; s < kSteps; ++s)
+      load_words<T, 4, A>(base + 64 * s, offset, (4 * s + g) * 4, width, reinterpret_cast<uint32_t*>(&out[s]));
   }
   static __device__ __forceinline__ int value_key(int g, int r) { return 4 * g + r; }
-  static __device__ __forceinline__ void scores(const u32x4* k, const u32x4* q, f32x4& s) {
+  template <int NQ, int NK>
+  static __device__ __forceinline__ void scores(const u32x4 (&k)[NK][kSteps], const u32x4 (&q)[NQ][kSteps], f32x4 (&s)[NQ][NK]) {
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i][e]), __uint_as_float(q[i][e]), s, 0, 0, 0);
+#pragma unroll
+        for (int t = 0; t < NQ; ++t)
+#pragma unroll
+          for (int u = 0; u < NK; ++u)
+            s[t][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[u][i][e]), __uint_as_float(q[t][i][e]),
+                                                           i + e ? s[t][u] : f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
   }
+  static constexpr uint32_t kSigns = 0x80000000u;
   template <int QT>
   static __device__ __forceinline__ void products(const Values& v, const f32x4 (&p)[QT][kTiles], f32x4 (&o)[QT][C]) {
 #pragma unroll
@@ -213,14 +229,16 @@ struct Args {
   const float* scale;
   void* out;
   float2* part;  // [ranges][kv head][row]: maximum, sum
-  float* sums;   // [ranges][kv head][row][width]: unnormalised output
-  float2* whole; // [kv head][row]: maximum, 1 / sum; null unless the weights are wanted
+  float* sums;   // [ranges][kv head][row][pitch]: unnormalised output
+  float2* whole; // [kv head][row]: maximum, 1 / sum
+  float* scores; // [batch][kv head][seq row][score_pitch]: own scores before the scale, or null
   const float* weights;
   float* weights_out;
   uint32_t batch, rows, q_heads, kv_heads, group, width, prefix, capacity;
   uint32_t seq_rows, all_rows;          // rows of one sequence and of the batch, per KV head
   uint32_t prefix_splits, own_splits;   // most ranges of a source
   uint32_t prefix_blocks, prefix_tiles, own_tiles;
+  uint32_t pitch, score_pitch;          // row widths of `sums` and `scores`
 };
 
 __device__ __forceinline__ uint32_t length_of(const Args& a, uint32_t b) {
@@ -245,67 +263,56 @@ __device__ __forceinline__ bool block_task(uint32_t id, uint32_t groups, uint32_
   return group < groups;
 }
 
+// The scale in units of ln 2; its sign goes into the query.
+__device__ __forceinline__ float factor_of(float scale) { return fabsf(scale) * kLog2e; }
+template <class Ops, int N>
+__device__ __forceinline__ void take_sign(float scale, u32x4 (&q)[N]) {
+  if (scale < 0.0f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = q[i] ^ Ops::kSigns;
+  }
+}
+
+// Wavefronts per SIMD that a kernel's registers are held to.
+template <class T, int D, int QT>
+constexpr int waves_per_simd() {
+  return D == 64 ? (QT == 1 ? 4 : QT == 2 ? 3 : 2) : D == 128 ? (QT == 4 ? 1 : 2) : 1;
+}
+
+// What a workgroup does: rows [first, first + count) of the batch's per KV head
+// against keys [begin, end) of one source, the result of range `slot`.
+struct Range {
+  const char *keys, *values;  // the KV head's features of the source's first key
+  float* scores;              // of the first row, or null
+  uint32_t first, count, kvh, begin, end, slot;
+  uint32_t least;             // keys that every row sees
+};
+
+template <class T, int D, int QT>
+struct Room {
+  static constexpr int C = D / 16;
+  f32x4 joined[QT == 1 ? 4 : 2 * QT][C][64];
+  float2 stats[2][QT][16];
+  float masked_p[kWaves][sizeof(T) == 2 ? 32 : 16][16];
+};
+
 template <class T, int D, int QT, Access A>
-__global__ __launch_bounds__(kThreads) void k_ranges(const Args a) {
+__device__ __forceinline__ void run_range(const Args& a, const Range& range, const uint32_t (&limit)[QT], Room<T, D, QT>& room) {
   using Ops = Operands<T, D, A>;
   constexpr int C = Ops::C, KT = Ops::kKeys, kTiles = Ops::kTiles;
-  __shared__ __align__(16) f32x4 joined[QT == 1 ? 4 : 2 * QT][C][64];
-  __shared__ float2 stats[2][QT][16];
-  __shared__ float masked_p[kWaves][KT][16];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int i16 = lane % 16, g = lane / 16;
-
-  // The rows [first, first + count) of the batch's per KV head, the keys
-  // [begin, end) of a source, and where the range's result goes.
-  uint32_t first, count, kvh, begin, end, slot, group, tile;
-  uint32_t limit[QT], least;
-  const T *keys, *values;
-  const uint32_t id = blockIdx.x;
-  if (id < a.prefix_blocks) {
-    if (!block_task(id, a.kv_heads * a.prefix_splits, a.prefix_tiles, group, tile)) return;
-    kvh = group % a.kv_heads;
-    slot = group / a.kv_heads;
-    const uint32_t each = range_keys(a.prefix, a.prefix_splits);
-    begin = slot * each;
-    if (begin >= a.prefix) return;
-    end = min(begin + each, a.prefix);
-    first = tile * 16 * QT;
-    count = min(a.all_rows - first, 16u * QT);
-    keys = static_cast<const T*>(a.prefix_key);
-    values = static_cast<const T*>(a.prefix_value);
-    least = end;
-#pragma unroll
-    for (int t = 0; t < QT; ++t) limit[t] = end;
-  } else {
-    if (!block_task(id - a.prefix_blocks, a.batch * a.kv_heads * a.own_splits, a.own_tiles, group, tile)) return;
-    kvh = group % a.kv_heads;
-    const uint32_t split = group / a.kv_heads % a.own_splits, b = group / a.kv_heads / a.own_splits;
-    slot = a.prefix_splits + split;
-    const uint32_t n = length_of(a, b), each = range_keys(n, a.own_splits);
-    begin = split * each;
-    if (begin >= n) return;
-    end = min(begin + each, n);
-    first = tile * 16 * QT;
-    count = min(a.seq_rows - first, 16u * QT);
-    least = min(end, visible(n, a.rows, first / a.group));
-    end = min(end, max(begin, visible(n, a.rows, (first + count - 1) / a.group)));  // no row sees further
-#pragma unroll
-    for (int t = 0; t < QT; ++t) limit[t] = visible(n, a.rows, min(first + 16 * t + i16, first + count - 1) / a.group);
-    first += b * a.seq_rows;
-    const uint64_t at = static_cast<uint64_t>(b) * a.capacity * a.kv_heads * a.width;
-    keys = static_cast<const T*>(a.key) + at;
-    values = static_cast<const T*>(a.value) + at;
-  }
-  const uint32_t stride = a.kv_heads * a.width;
   const int width = a.width;
-  keys += static_cast<uint64_t>(kvh) * width;
-  values += static_cast<uint64_t>(kvh) * width;
-  const float scale = *a.scale;
+  const uint32_t stride = a.kv_heads * a.width * sizeof(T), end = range.end;
+  const float scale = *a.scale, factor = factor_of(scale);
 
   u32x4 q[QT][Ops::kSteps];
 #pragma unroll
-  for (int t = 0; t < QT; ++t)
-    Ops::load_row(static_cast<const T*>(a.query) + query_offset(a, first + min(16u * t + i16, count - 1), kvh), g, width, q[t]);
+  for (int t = 0; t < QT; ++t) {
+    const uint64_t at = query_offset(a, range.first + min(16u * t + i16, range.count - 1), range.kvh);
+    Ops::load_row(reinterpret_cast<const char*>(static_cast<const T*>(a.query) + at), 16 * g, g, width, q[t]);
+    take_sign<Ops>(scale, q[t]);
+  }
 
   f32x4 o[QT][C];
   float top[QT], sum[QT];
@@ -317,91 +324,102 @@ __global__ __launch_bounds__(kThreads) void k_ranges(const Args a) {
     for (int j = 0; j < C; ++j) o[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  typename Ops::Keys kf;
+  u32x4 kf[kTiles][Ops::kSteps];
   typename Ops::Values vf;
-  // Rows past the last key repeat it: they are masked, and their values cleared.
+  // A step's rows by 32-bit offsets from its first key; rows past the last key
+  // repeat it: they are masked, and their values cleared.
+  const uint32_t key_offset = i16 * stride + 16 * g;
+  const uint32_t value_offset = 4 * g * stride + i16 * C * sizeof(T);
   auto load_keys = [&](uint32_t at) {
-    const T* base = keys + static_cast<uint64_t>(at) * stride;
-    const uint32_t last = end - at - 1;
+    const char* base = range.keys + static_cast<uint64_t>(at) * stride;
+    const uint32_t most = min(end - at - 1, 63u) * stride + 16 * g;
 #pragma unroll
-    for (int u = 0; u < kTiles; ++u) Ops::load_row(base + min(16u * u + i16, last) * stride, g, width, kf.v[u]);
+    for (int u = 0; u < kTiles; ++u) Ops::load_row(base, min(key_offset + 16 * u * stride, most), g, width, kf[u]);
   };
   auto load_values = [&](uint32_t at) {
-    const T* base = values + static_cast<uint64_t>(at) * stride;
-    const uint32_t last = end - at - 1;
+    const char* base = range.values + static_cast<uint64_t>(at) * stride;
+    const uint32_t most = min(end - at - 1, 63u) * stride + i16 * C * sizeof(T);
 #pragma unroll
     for (int r = 0; r < Ops::kValueRows; ++r)
-      load_words<T, C, A>(base + min(static_cast<uint32_t>(Ops::value_key(g, r)), last) * stride, i16 * C, width, vf.v[r]);
+      load_words<T, C, A>(base, min(value_offset + Ops::value_key(0, r) * stride, most), i16 * C, width, vf.v[r]);
   };
-
   // The elements of the step's first `seen` keys that are not finite, added to
   // the lane's row of outputs in `joined`.
-  auto add_special = [&](const T* row, uint32_t row_stride, uint32_t seen) {
-    for (uint32_t k = 0; k < seen; ++k, row += row_stride) {
-      const float share = masked_p[wave][k][i16];
+  auto add_special = [&](const char* row, uint32_t seen) {
+    for (uint32_t k = 0; k < seen; ++k, row += stride) {
+      const float share = room.masked_p[wave][k][i16];
 #pragma unroll 1
       for (int m = 0; m < 4 * C; ++m) {
         const int f = 4 * g * C + m;
-        const float v = f < width ? load_elem(row, f) : 0.0f;
-        float& to = reinterpret_cast<float*>(&joined[wave][m % C][lane])[m / C];
+        const float v = f < width ? load_elem(reinterpret_cast<const T*>(row), f) : 0.0f;
+        float& to = reinterpret_cast<float*>(&room.joined[wave][m % C][lane])[m / C];
         if (!(fabsf(v) < INFINITY)) to = fma_rn(share, v, to);
       }
     }
   };
 
-  // Steps past the range repeat its last key: operands stay defined on every path.
-  uint32_t at = begin + wave * KT;
+  // Steps past the range repeat its last key: operands are defined on every
+  // path.  (With the loads under a condition the compiler has reused part of
+  // a loaded row's registers before its last use.)
+  uint32_t at = range.begin + wave * KT;
   if (at < end) {
     load_keys(at);
     load_values(at);
   }
   while (at < end) {
-    const uint32_t next = at + kWaves * KT;
+    const uint32_t next = at + kWaves * KT, ahead = min(next, end - 1);
     f32x4 p[QT][kTiles];
+    Ops::scores(kf, q, p);
+    load_keys(ahead);
+    if (range.scores) {
+      float* row = range.scores + static_cast<uint64_t>(i16) * a.score_pitch + at + 4 * g;
+      if (static_cast<uint32_t>(i16) < range.count) {
 #pragma unroll
-    for (int t = 0; t < QT; ++t)
-#pragma unroll
-      for (int u = 0; u < kTiles; ++u) {
-        p[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        Ops::scores(kf.v[u], q[t], p[t][u]);
+        for (int u = 0; u < kTiles; ++u) *reinterpret_cast<f32x4*>(row + 16 * u) = p[0][u];
       }
-    load_keys(min(next, end - 1));
-    const bool masked = at + KT > least;
+    }
+    const bool masked = at + KT > range.least;
+    if (masked) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (at + 16 * u + 4 * g + r >= limit[t]) p[t][u][r] = -INFINITY;
+    }
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       float most = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < kTiles; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float s = p[t][u][r] * scale;
-          if (masked && at + 16 * u + 4 * g + r >= limit[t]) s = -INFINITY;
-          p[t][u][r] = s;
-          most = fmaxf(most, s);
-        }
-      if (__any(most > top[t] + kSlack)) {
-        const float raised = fmaxf(top[t], group_max(most));
-        const float factor = top[t] == -INFINITY ? 1.0f : fast_exp(top[t] - raised);  // nothing summed yet: zeros
+      for (int u = 0; u < kTiles; ++u) most = fmaxf(most, fmaxf(fmaxf(p[t][u][0], p[t][u][1]), fmaxf(p[t][u][2], p[t][u][3])));
+      if (__any(most * factor > top[t] + kSlack)) {
+        const float raised = fmaxf(top[t], group_max(most) * factor);
+        const float less = top[t] == -INFINITY ? 1.0f : exp2_of(top[t] - raised);  // nothing summed yet: zeros
         top[t] = raised;
-        sum[t] = sum[t] * factor;
+        sum[t] = sum[t] * less;
 #pragma unroll
-        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * factor;
+        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * less;
       }
-      const float from = reference_of(top[t]);
+      const float from = -reference_of(top[t]);
 #pragma unroll
       for (int u = 0; u < kTiles; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[t][u][r] = fast_exp(p[t][u][r] - from);
-          sum[t] = sum[t] + p[t][u][r];
-        }
+        for (int r = 0; r < 4; ++r) p[t][u][r] = exp2_of(fma_rn(p[t][u][r], factor, from));
     }
     if (masked) {
-      // Values of keys past the end are cleared.  An infinity or NaN in the
-      // values of a key that only some rows see must not reach the others
-      // through 0 * inf: such elements leave the product and are added row by
-      // row.
+      // A score of a zero or NaN scale must not reach a hidden key.  Values of
+      // keys past the end are cleared.  An infinity or NaN in the values of a
+      // key that only some rows see must not reach the others through 0 * inf:
+      // such elements leave the product and are added row by row.
       bool special = false;
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (at + 16 * u + 4 * g + r >= limit[t]) p[t][u][r] = 0.0f;
 #pragma unroll
       for (int r = 0; r < Ops::kValueRows; ++r)
 #pragma unroll
@@ -417,47 +435,55 @@ __global__ __launch_bounds__(kThreads) void k_ranges(const Args a) {
 #pragma unroll
           for (int u = 0; u < kTiles; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) masked_p[wave][16 * u + 4 * g + r][i16] = p[t][u][r];
+            for (int r = 0; r < 4; ++r) room.masked_p[wave][16 * u + 4 * g + r][i16] = p[t][u][r];
 #pragma unroll
-          for (int j = 0; j < C; ++j) joined[wave][j][lane] = o[t][j];
+          for (int j = 0; j < C; ++j) room.joined[wave][j][lane] = o[t][j];
           __builtin_amdgcn_wave_barrier();
-          add_special(values + static_cast<uint64_t>(at) * stride, stride, min(min(limit[t], end), at + KT) - at);
+          const uint32_t seen = min(min(limit[t], end), at + KT);
+          add_special(range.values + static_cast<uint64_t>(at) * stride, seen > at ? seen - at : 0);
           __builtin_amdgcn_wave_barrier();
 #pragma unroll
-          for (int j = 0; j < C; ++j) o[t][j] = joined[wave][j][lane];
+          for (int j = 0; j < C; ++j) o[t][j] = room.joined[wave][j][lane];
         }
       }
     }
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int u = 0; u < kTiles; ++u) sum[t] = sum[t] + ((p[t][u][0] + p[t][u][1]) + (p[t][u][2] + p[t][u][3]));
     Ops::template products<QT>(vf, p, o);
-    load_values(min(next, end - 1));
+    load_values(ahead);
     at = next;
   }
 #pragma unroll
   for (int t = 0; t < QT; ++t) sum[t] = group_sum(sum[t]);
 
-  // Join the wavefronts: 2 and 3 into 0 and 1, then 1 into 0.
+  // Join the wavefronts: 2 and 3 into 0 and 1, then 1 into 0; those without a
+  // step have nothing to give.
+  const uint32_t steps = end > range.begin ? (end - range.begin + KT - 1) / KT : 0;
   __syncthreads();
 #pragma unroll
   for (int half = 2; half; half /= 2) {
+    if (steps <= static_cast<uint32_t>(half)) continue;
     if (wave >= half && wave < 2 * half) {
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        if (g == 0) stats[wave - half][t][i16] = make_float2(top[t], sum[t]);
+        if (g == 0) room.stats[wave - half][t][i16] = make_float2(top[t], sum[t]);
 #pragma unroll
-        for (int j = 0; j < C; ++j) joined[(wave - half) * QT + t][j][lane] = o[t][j];
+        for (int j = 0; j < C; ++j) room.joined[(wave - half) * QT + t][j][lane] = o[t][j];
       }
     }
     __syncthreads();
     if (wave < half) {
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        const float2 other = stats[wave][t][i16];
-        const float raised = reference_of(fmaxf(top[t], other.x));
-        const float mine = fast_exp(top[t] - raised), theirs = fast_exp(other.x - raised);
-        top[t] = fmaxf(top[t], other.x);
+        const float2 other = room.stats[wave][t][i16];
+        const float raised = fmaxf(top[t], other.x), from = reference_of(raised);
+        const float mine = exp2_of(top[t] - from), theirs = exp2_of(other.x - from);
+        top[t] = raised;
         sum[t] = fma_rn(sum[t], mine, other.y * theirs);
 #pragma unroll
-        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * mine + joined[wave * QT + t][j][lane] * theirs;
+        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * mine + room.joined[wave * QT + t][j][lane] * theirs;
       }
     }
     __syncthreads();
@@ -466,128 +492,261 @@ __global__ __launch_bounds__(kThreads) void k_ranges(const Args a) {
   // A lane holds features 4 C g .. of its row, 4 C of them in order.
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    if (16u * t + i16 >= count) continue;
-    const uint64_t row = (static_cast<uint64_t>(slot) * a.kv_heads + kvh) * a.all_rows + first + 16 * t + i16;
+    if (16u * t + i16 >= range.count) continue;
+    const uint64_t row = (static_cast<uint64_t>(range.slot) * a.kv_heads + range.kvh) * a.all_rows + range.first + 16 * t + i16;
     if (g == 0) a.part[row] = make_float2(top[t], sum[t]);
-    float* dst = a.sums + row * width;
+    float* dst = a.sums + row * a.pitch;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int m = 0; m < C; ++m) {
+      const uint32_t f = 4 * (g * C + m);
+      f32x4 v;
 #pragma unroll
-      for (int j = 0; j < C; ++j) {
-        const int f = (4 * g + r) * C + j;
-        if (A == Access::kWhole || f < width) dst[f] = o[t][j][r];
-      }
+      for (int e = 0; e < 4; ++e) v[e] = o[t][(4 * m + e) % C][(4 * m + e) / C];
+      if (A == Access::kWhole || f < a.pitch) *reinterpret_cast<f32x4*>(dst + f) = v;
+    }
   }
 }
 
-// Joins the ranges of one row: a wavefront per (KV head, row), the ranges'
-// maxima and sums across its lanes, then their outputs one after the other.
-template <class T>
-__global__ __launch_bounds__(kThreads) void k_join(const Args a) {
-  const int lane = threadIdx.x % 64;
-  const uint32_t task = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  if (task >= a.kv_heads * a.all_rows) return;
+// QP row tiles per workgroup against the prefix, QO against an own cache: a
+// sequence of a decode step has few rows where the batch has many.
+template <class T, int D, int QP, int QO, Access A>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(waves_per_simd<T, D, QP>())))
+void k_ranges(const Args a) {
+  __shared__ __align__(16) Room<T, D, QP> room;
+  const int i16 = threadIdx.x % 16;
+  const uint64_t stride = static_cast<uint64_t>(a.kv_heads) * a.width;
+  Range range;
+  uint32_t group, tile;
+  if (blockIdx.x < a.prefix_blocks) {
+    if (!block_task(blockIdx.x, a.kv_heads * a.prefix_splits, a.prefix_tiles, group, tile)) return;
+    range.kvh = group % a.kv_heads;
+    range.slot = group / a.kv_heads;
+    const uint32_t each = range_keys(a.prefix, a.prefix_splits);
+    range.begin = range.slot * each;
+    if (range.begin >= a.prefix) return;
+    range.end = range.least = min(range.begin + each, a.prefix);
+    range.first = tile * 16 * QP;
+    range.count = min(a.all_rows - range.first, 16u * QP);
+    range.scores = nullptr;
+    const uint64_t at = static_cast<uint64_t>(range.kvh) * a.width * sizeof(T);
+    range.keys = static_cast<const char*>(a.prefix_key) + at;
+    range.values = static_cast<const char*>(a.prefix_value) + at;
+    uint32_t limit[QP];
+#pragma unroll
+    for (int t = 0; t < QP; ++t) limit[t] = range.end;
+    run_range<T, D, QP, A>(a, range, limit, room);
+    return;
+  }
+  if (!block_task(blockIdx.x - a.prefix_blocks, a.batch * a.kv_heads * a.own_splits, a.own_tiles, group, tile)) return;
+  range.kvh = group % a.kv_heads;
+  const uint32_t split = group / a.kv_heads % a.own_splits, b = group / a.kv_heads / a.own_splits;
+  range.slot = a.prefix_splits + split;
+  const uint32_t n = length_of(a, b), each = range_keys(n, a.own_splits);
+  range.begin = split * each;
+  if (range.begin >= n) return;
+  const uint32_t first = tile * 16 * QO;
+  range.count = min(a.seq_rows - first, 16u * QO);
+  range.end = min(range.begin + each, n);
+  range.least = min(range.end, visible(n, a.rows, first / a.group));
+  range.end = min(range.end, max(range.begin, visible(n, a.rows, (first + range.count - 1) / a.group)));  // no row sees further
+  uint32_t limit[QO];
+#pragma unroll
+  for (int t = 0; t < QO; ++t) limit[t] = visible(n, a.rows, min(first + 16 * t + i16, first + range.count - 1) / a.group);
+  range.first = b * a.seq_rows + first;
+  range.scores = a.scores ? a.scores + ((static_cast<uint64_t>(b) * a.kv_heads + range.kvh) * a.seq_rows + first) * a.score_pitch : nullptr;
+  const uint64_t at = (b * a.capacity * stride + static_cast<uint64_t>(range.kvh) * a.width) * sizeof(T);
+  range.keys = static_cast<const char*>(a.key) + at;
+  range.values = static_cast<const char*>(a.value) + at;
+  run_range<T, D, QO, A>(a, range, limit, reinterpret_cast<Room<T, D, QO>&>(room));
+}
+
+// The ranges that hold something of one row, in order.
+struct RowRanges {
+  uint32_t before, own, seen;
+  uint64_t step, base;
+  __device__ __forceinline__ RowRanges(const Args& a, uint32_t kvh, uint32_t row, uint32_t n) {
+    seen = visible(n, a.rows, row % a.seq_rows / a.group);
+    before = ranges_of(a.prefix, a.prefix_splits);
+    own = seen ? (seen - 1) / range_keys(n, a.own_splits) + 1 : 0;  // ranges past the last key it sees hold nothing of it
+    step = static_cast<uint64_t>(a.kv_heads) * a.all_rows;
+    base = static_cast<uint64_t>(kvh) * a.all_rows + row;
+    skipped = a.prefix_splits - before;
+  }
+  __device__ __forceinline__ uint32_t count() const { return before + own; }
+  __device__ __forceinline__ uint64_t place(uint32_t r) const { return (r < before ? r : r + skipped) * step + base; }
+  // Maximum (as subtracted) and sum over all ranges, by one wavefront.
+  __device__ __forceinline__ float2 whole(const float2* part) const {
+    const uint32_t lane = threadIdx.x % 64;
+    float top = -INFINITY;
+    for (uint32_t r = lane; r < count(); r += 64) top = fmaxf(top, part[place(r)].x);
+    const float from = reference_of(wave_max(top));
+    float total = 0.0f;
+    for (uint32_t r = lane; r < count(); r += 64) {
+      const float2 p = part[place(r)];
+      total = fma_rn(exp2_of(p.x - from), p.y, total);
+    }
+#pragma unroll
+    for (int off = 32; off; off /= 2) total = total + __shfl_xor(total, off);
+    return make_float2(from, total);
+  }
+
+ private:
+  uint32_t skipped;
+};
+
+// Joins the ranges of one row.  D / 4 lanes hold a row of a range, four
+// features each, so a wavefront reads 256 / D ranges at a time and a workgroup
+// of W = 4 four times as many: the loads of a row are a few deep.
+template <class T, int D, int W>
+__device__ __forceinline__ void join_row(const Args& a, uint32_t task, f32x4 (*room)[64]) {
+  constexpr int kLanes = D / 4, kAtOnce = W * 64 / kLanes;
+  const int lane = threadIdx.x % 64, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t kvh = task % a.kv_heads, row = task / a.kv_heads;
-  const uint32_t b = row / a.seq_rows, n = length_of(a, b), seen = visible(n, a.rows, row % a.seq_rows / a.group);
-  const uint32_t before = ranges_of(a.prefix, a.prefix_splits);
-  const uint32_t each = range_keys(n, a.own_splits);
-  const uint32_t own = seen ? (seen - 1) / each + 1 : 0;  // ranges past the last key it sees hold nothing of it
-  const uint32_t ranges = before + own;
-  const uint64_t step = static_cast<uint64_t>(a.kv_heads) * a.all_rows;
-  const uint64_t base = static_cast<uint64_t>(kvh) * a.all_rows + row;
-  auto place = [&](uint32_t r) { return (r < before ? r : a.prefix_splits + r - before) * step + base; };
-  T* out = static_cast<T*>(a.out) + query_offset(a, row, kvh);
-  float top = -INFINITY;
-  for (uint32_t r = lane; r < ranges; r += 64) top = fmaxf(top, a.part[place(r)].x);
-  top = wave_max(top);
-  const float from = reference_of(top);
-  float total = 0.0f;
-  float acc[4] = {};
-  for (uint32_t r0 = 0; r0 < ranges; r0 += 64) {
-    float factor = 0.0f;
-    if (r0 + lane < ranges) {
-      const float2 part = a.part[place(r0 + lane)];
-      factor = fast_exp(part.x - from);
-      total = fma_rn(factor, part.y, total);
-    }
-    const uint32_t some = min(ranges - r0, 64u);
-    for (uint32_t r = 0; r < some; ++r) {
-      const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(factor), r));
-      const float* src = a.sums + place(r0 + r) * a.width;
+  const RowRanges ranges(a, kvh, row, length_of(a, row / a.seq_rows));
+  const uint32_t f = lane % kLanes * 4, first = wave * (64 / kLanes) + lane / kLanes;
+  const float2 whole = ranges.whole(a.part);
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (f < a.pitch) {
+#pragma unroll 4
+    for (uint32_t r = first; r < ranges.count(); r += kAtOnce) {
+      const uint64_t at = ranges.place(r);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a.sums + at * a.pitch + f);
+      const float share = exp2_of(a.part[at].x - whole.x);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (lane + 64u * k < a.width) acc[k] = fma_rn(f, src[lane + 64 * k], acc[k]);
+      for (int e = 0; e < 4; ++e) acc[e] = fma_rn(share, v[e], acc[e]);
     }
   }
 #pragma unroll
-  for (int off = 32; off; off /= 2) total = total + __shfl_xor(total, off);
-  const bool none = a.prefix + seen == 0;
+  for (int off = kLanes; off < 64; off *= 2)
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (lane + 64u * k < a.width) store_elem(out, lane + 64 * k, none ? 0.0f : acc[k] / total);
-  if (a.whole && lane == 0) a.whole[base] = make_float2(from, 1.0f / total);
+    for (int e = 0; e < 4; ++e) acc[e] = acc[e] + __shfl_xor(acc[e], off);
+  if constexpr (W > 1) {
+    room[wave][lane] = acc;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) acc = acc + room[w][lane];
+  }
+  if (lane == 0) a.whole[ranges.base] = make_float2(whole.x, 1.0f / whole.y);
+  if (lane >= kLanes) return;
+  T* out = static_cast<T*>(a.out) + query_offset(a, row, kvh);
+  const bool none = a.prefix + ranges.seen == 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (f + e < a.width) store_elem(out, f + e, none ? 0.0f : acc[e] / whole.y);
 }
 
-// Weights: a wavefront holds 16 keys and walks the rows that see them,
-// computing the scores again; a lane sums its 4 keys over its rows, then the
-// 16 lanes of a key add up.  Every key has one owner: no atomics.
+// Weights of up to 16 rows from their stored scores: a thread sums four
+// keys' weights over the rows.
+constexpr int kWeightKeys = 4 * kThreads;
+__device__ __forceinline__ void add_weights(const Args& a, uint32_t block, float2* stats) {
+  const uint32_t blocks = a.capacity / kWeightKeys + (a.capacity % kWeightKeys != 0);
+  const uint32_t kvh = block % a.kv_heads, b = block / a.kv_heads / blocks;
+  const uint32_t key0 = block / a.kv_heads % blocks * kWeightKeys;
+  const uint32_t n = length_of(a, b);
+  if (key0 >= n) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  for (uint32_t r = wave; r < a.seq_rows; r += kWaves) {
+    const float2 whole = RowRanges(a, kvh, b * a.seq_rows + r, n).whole(a.part);
+    if (threadIdx.x % 64 == 0) stats[r] = make_float2(whole.x, 1.0f / whole.y);
+  }
+  __syncthreads();
+  const float factor = factor_of(*a.scale);
+  const uint32_t key = key0 + 4 * threadIdx.x;
+  if (key >= n) return;
+  const uint64_t head = static_cast<uint64_t>(b) * a.kv_heads + kvh;
+  const float* scores = a.scores + head * a.seq_rows * a.score_pitch + key;
+  float sum[4] = {};
+#pragma unroll 4
+  for (uint32_t r = 0; r < a.seq_rows; ++r) {
+    const f32x4 s = *reinterpret_cast<const f32x4*>(scores + static_cast<uint64_t>(r) * a.score_pitch);
+    const uint32_t seen = visible(n, a.rows, r / a.group);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (key + e < seen) sum[e] = fma_rn(exp2_of(fma_rn(s[e], factor, -stats[r].x)), stats[r].y, sum[e]);
+  }
+  const uint64_t at = head * a.capacity + key;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (key + e < n) a.weights_out[at + e] = a.weights[at + e] + sum[e];
+}
+
+template <class T, int D, int W>
+__global__ __launch_bounds__(kThreads) void k_join(const Args a, uint32_t join_blocks) {
+  __shared__ f32x4 room[W == 1 ? 1 : W][64];
+  __shared__ float2 stats[16];
+  if (blockIdx.x < join_blocks) {
+    const uint32_t task = W == 1 ? blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : blockIdx.x;
+    if (task < a.kv_heads * a.all_rows) join_row<T, D, W>(a, task, room);
+  } else {
+    add_weights(a, blockIdx.x - join_blocks, stats);
+  }
+}
+
+// Weights of more rows: the scores again, a workgroup per 16 NT keys, held in
+// registers.  The wavefronts walk every fourth tile of the rows that see them;
+// a lane sums its keys over its rows, then the lanes and the wavefronts add up
+// in a fixed order.  Every key has one owner: no atomics.
 template <class T, int D, Access A>
 __global__ __launch_bounds__(kThreads) void k_weights(const Args a) {
   using Ops = Operands<T, D, A>;
+  constexpr int NT = D == 256 ? 2 : 4, kKeys = 16 * NT;
+  __shared__ float sums[kWaves][kKeys];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int i16 = lane % 16, g = lane / 16;
-  const uint32_t blocks = a.capacity / 64 + (a.capacity % 64 != 0);
+  const uint32_t blocks = a.capacity / kKeys + (a.capacity % kKeys != 0);
   const uint32_t kvh = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads / blocks;
-  const uint32_t key0 = blockIdx.x / a.kv_heads % blocks * 64 + wave * 16;
+  const uint32_t key0 = blockIdx.x / a.kv_heads % blocks * kKeys;
   const uint32_t n = length_of(a, b);
   if (key0 >= n) return;
-  const uint32_t stride = a.kv_heads * a.width;
-  const T* keys = static_cast<const T*>(a.key) + (static_cast<uint64_t>(b) * a.capacity + key0) * stride +
-                  static_cast<uint64_t>(kvh) * a.width;
-  u32x4 k[Ops::kSteps];
-  Ops::load_row(keys + min(static_cast<uint32_t>(i16), n - key0 - 1) * stride, g, a.width, k);
-  const float scale = *a.scale;
-  float sum[4] = {};
+  const uint32_t stride = a.kv_heads * a.width * sizeof(T);
+  const char* keys = static_cast<const char*>(a.key) + (static_cast<uint64_t>(b) * a.capacity + key0) * stride +
+                     static_cast<uint64_t>(kvh) * a.width * sizeof(T);
+  const float scale = *a.scale, factor = factor_of(scale);
+  u32x4 k[NT][Ops::kSteps];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) Ops::load_row(keys, min(16u * u + i16, n - key0 - 1) * stride + 16 * g, g, a.width, k[u]);
+  float sum[NT][4] = {};
   // The first row that sees key0: n - rows + i + 1 > key0.
-  const uint64_t from_row = static_cast<uint64_t>(key0) + a.rows > n ? key0 + a.rows - n : 0;
-  for (uint32_t r0 = static_cast<uint32_t>(from_row) * a.group / 16 * 16; r0 < a.seq_rows; r0 += 16) {
+  const uint32_t from_row = static_cast<uint64_t>(key0) + a.rows > n ? key0 + a.rows - n : 0;
+  for (uint32_t r0 = from_row * a.group / 16 * 16 + 16 * wave; r0 < a.seq_rows; r0 += 16 * kWaves) {
     const uint32_t in_seq = min(r0 + i16, a.seq_rows - 1), row = b * a.seq_rows + in_seq;
-    u32x4 q[Ops::kSteps];
-    Ops::load_row(static_cast<const T*>(a.query) + query_offset(a, row, kvh), g, a.width, q);
+    u32x4 q[1][Ops::kSteps];
+    Ops::load_row(reinterpret_cast<const char*>(static_cast<const T*>(a.query) + query_offset(a, row, kvh)), 16 * g, g, a.width, q[0]);
+    take_sign<Ops>(scale, q[0]);
     const float2 whole = a.whole[static_cast<uint64_t>(kvh) * a.all_rows + row];
-    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 s[1][NT];
     Ops::scores(k, q, s);
     const uint32_t seen = r0 + i16 < a.seq_rows ? visible(n, a.rows, in_seq / a.group) : 0;
+    const bool all = __all(seen >= key0 + kKeys);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (key0 + 4 * g + r < seen) sum[r] = sum[r] + fast_exp(s[r] * scale - whole.x) * whole.y;
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float share = exp2_of(fma_rn(s[0][u][r], factor, -whole.x)) * whole.y;
+        if (all || key0 + 16 * u + 4 * g + r < seen) sum[u][r] = sum[u][r] + share;
+      }
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
+  for (int u = 0; u < NT; ++u)
 #pragma unroll
-    for (int off = 8; off; off /= 2) sum[r] = sum[r] + __shfl_xor(sum[r], off);
-    const uint32_t key = key0 + 4 * g + r;
-    if (i16 == 0 && key < n) {
-      const uint64_t at = (static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.capacity + key;
-      a.weights_out[at] = a.weights[at] + sum[r];
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+      for (int off = 8; off; off /= 2) sum[u][r] = sum[u][r] + __shfl_xor(sum[u][r], off);
+      if (i16 == 0) sums[wave][16 * u + 4 * g + r] = sum[u][r];
     }
+  __syncthreads();
+  const uint32_t key = key0 + threadIdx.x;
+  if (threadIdx.x < kKeys && key < n) {
+    const uint64_t at = (static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.capacity + key;
+    const float* own = &sums[0][threadIdx.x];
+    a.weights_out[at] = a.weights[at] + ((own[0] + own[kKeys]) + (own[2 * kKeys] + own[3 * kKeys]));
   }
 }
 
 // ------------------------------------------------------------------- the host
 constexpr const char* kTooMany = "too many workgroups";
-
-// Row tiles per workgroup, ranges and workspace of one call.
-struct Layout {
-  Args args{};
-  int tiles = 1;  // QT
-  int features = 64;  // D
-  uint64_t part_bytes = 0, sums_bytes = 0, whole_bytes = 0;
-  uint32_t own_blocks = 0;
-  uint64_t bytes() const { return part_bytes + sums_bytes + whole_bytes; }
-  void set_tiles(int count);
-  void count_blocks();
-};
+constexpr uint64_t kMostBlocks = 1u << 30;
 
 uint64_t product(std::initializer_list<uint64_t> factors, uint64_t most, const char* what) {
   uint64_t p = 1;
@@ -598,20 +757,34 @@ uint64_t product(std::initializer_list<uint64_t> factors, uint64_t most, const c
   return p;
 }
 
-void Layout::set_tiles(int count) {
-  tiles = count;
-  args.prefix_tiles = static_cast<uint32_t>(ceil_div(args.all_rows, 16 * count));
-  args.own_tiles = static_cast<uint32_t>(ceil_div(args.seq_rows, 16 * count));
-}
+// Row tiles per workgroup, ranges and workspace of one call.
+struct Layout {
+  Args args{};
+  int prefix_q = 1, own_q = 1;  // row tiles of 16
+  int features = 64;            // D
+  bool weighted = false, stored = false;
+  uint64_t part_bytes = 0, sums_bytes = 0, whole_bytes = 0, score_bytes = 0;
+  uint32_t own_blocks = 0, weight_blocks = 0;
 
-void Layout::count_blocks() {
-  constexpr uint64_t kMost = 1u << 30;
-  auto blocks = [&](std::initializer_list<uint64_t> groups, uint64_t tile_count) {
-    return static_cast<uint32_t>(product({ceil_div(product(groups, kMost, kTooMany), 8) * 8, tile_count}, kMost, kTooMany));
-  };
-  args.prefix_blocks = blocks({args.kv_heads, args.prefix_splits}, args.prefix_tiles);
-  own_blocks = blocks({args.batch, args.kv_heads, args.own_splits}, args.own_tiles);
-}
+  uint64_t bytes() const { return part_bytes + sums_bytes + whole_bytes + score_bytes; }
+  void set_tiles(int prefix, int own) {
+    prefix_q = prefix;
+    own_q = own;
+    args.prefix_tiles = static_cast<uint32_t>(ceil_div(args.all_rows, 16 * prefix));
+    args.own_tiles = static_cast<uint32_t>(ceil_div(args.seq_rows, 16 * own));
+  }
+  void count_blocks() {
+    auto blocks = [&](std::initializer_list<uint64_t> groups, uint64_t tiles) {
+      const uint64_t rounded = ceil_div(product(groups, kMostBlocks, kTooMany), 8) * 8;
+      return static_cast<uint32_t>(product({rounded, tiles}, kMostBlocks, kTooMany));
+    };
+    args.prefix_blocks = blocks({args.kv_heads, args.prefix_splits}, args.prefix_tiles);
+    own_blocks = blocks({args.batch, args.kv_heads, args.own_splits}, args.own_tiles);
+    const uint64_t keys = stored ? kWeightKeys : features == 256 ? 32 : 64;  // per block
+    weight_blocks = static_cast<uint32_t>(
+        weighted ? product({args.batch, args.kv_heads, ceil_div(args.capacity, keys)}, kMostBlocks, kTooMany) : 0);
+  }
+};
 
 Layout layout_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted) {
   check_shape(shape);
@@ -632,23 +805,32 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted) {
   a.all_rows = static_cast<uint32_t>(product({a.seq_rows, a.batch}, 1u << 30, kRows));
   product({a.all_rows, a.kv_heads}, 1u << 30, kRows);
   l.features = a.width <= 64 ? 64 : a.width <= 128 ? 128 : 256;
-  // Rows per workgroup: few rows leave no tile empty; D = 256 has room for two.
-  const uint32_t most_rows = prefix ? a.all_rows : a.seq_rows;
-  l.set_tiles(most_rows <= 16 ? 1 : most_rows <= 32 || l.features == 256 ? 2 : 4);
-  // Ranges: about kBlocks workgroups in all, each with whole rounds of keys.
-  constexpr uint64_t kBlocks = 512;
+  l.weighted = weighted;
+  l.stored = weighted && a.seq_rows <= 16;
+  // Rows per workgroup: as many tiles as the rows fill; D = 256 has registers
+  // for two.
+  auto tiles = [&](uint32_t rows) { return rows <= 16 ? 1 : rows <= 32 || l.features == 256 ? 2 : 4; };
+  const int own = tiles(a.seq_rows), all = prefix ? tiles(a.all_rows) : own;
+  l.set_tiles(all, own == 1 ? 1 : all);
+  // Ranges: as many workgroups as the chip holds at once, each with whole rounds of keys.
+  const uint64_t held = 256 * (l.features == 64 ? (all == 1 ? 4 : all == 2 ? 3 : 2) : l.features == 128 && all < 4 ? 2 : 1);
   const double work = static_cast<double>(a.kv_heads) *
                       (static_cast<double>(a.prefix_tiles) * a.prefix +
                        static_cast<double>(a.batch) * a.own_tiles * a.capacity);
-  const uint64_t each = std::max<uint64_t>(kRound, static_cast<uint64_t>(work / kBlocks));
+  const uint64_t each = std::max<uint64_t>(kRound, static_cast<uint64_t>(work / held));
   a.prefix_splits = static_cast<uint32_t>(ceil_div(prefix, each));
   a.own_splits = static_cast<uint32_t>(ceil_div(a.capacity, each));
   l.count_blocks();
-  const uint64_t ranges = a.prefix_splits + a.own_splits, most = UINT64_MAX / 8;
-  const uint64_t entries = product({ranges, a.kv_heads, a.all_rows}, most, "workspace too large");
-  l.part_bytes = ceil_div(product({entries, 8}, most, "workspace too large"), 256) * 256;
-  l.sums_bytes = ceil_div(product({entries, a.width, 4}, most, "workspace too large"), 256) * 256;
-  l.whole_bytes = weighted ? ceil_div(static_cast<uint64_t>(a.kv_heads) * a.all_rows * 8, 256) * 256 : 0;
+  a.pitch = (a.width + 3) / 4 * 4;
+  a.score_pitch = (a.capacity + 31) / 32 * 32;
+  constexpr const char* kLarge = "workspace too large";
+  constexpr uint64_t kMost = UINT64_MAX / 8;
+  auto room = [&](std::initializer_list<uint64_t> factors) { return ceil_div(product(factors, kMost, kLarge), 256) * 256; };
+  const uint64_t entries = product({uint64_t{a.prefix_splits} + a.own_splits, a.kv_heads, a.all_rows}, kMost, kLarge);
+  l.part_bytes = room({entries, 8});
+  l.sums_bytes = room({entries, a.pitch, 4});
+  l.whole_bytes = room({a.kv_heads, a.all_rows, 8});
+  l.score_bytes = l.stored ? room({a.kv_heads, a.all_rows, a.score_pitch, 4}) : 0;
   return l;
 }
 
@@ -656,19 +838,37 @@ template <class T, int D, Access A>
 void launch(hipStream_t s, const Layout& l) {
   const Args& a = l.args;
   const unsigned blocks = a.prefix_blocks + l.own_blocks;  // at most 2^31
-  if (l.tiles == 1) {
-    k_ranges<T, D, 1, A><<<blocks, kThreads, 0, s>>>(a);
+  auto run = [&](auto prefix_q, auto own_q) {
+    k_ranges<T, D, decltype(prefix_q)::value, decltype(own_q)::value, A><<<blocks, kThreads, 0, s>>>(a);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  using Four = std::integral_constant<int, 4>;
+  if (l.prefix_q == 1) {
+    run(One{}, One{});
   } else if constexpr (A != Access::kElements) {
-    if (l.tiles == 2)
-      k_ranges<T, D, 2, A><<<blocks, kThreads, 0, s>>>(a);
-    else if constexpr (D != 256)
-      k_ranges<T, D, 4, A><<<blocks, kThreads, 0, s>>>(a);
+    if (l.prefix_q == 2) {
+      if (l.own_q == 1)
+        run(Two{}, One{});
+      else
+        run(Two{}, Two{});
+    } else if constexpr (D != 256) {
+      if (l.own_q == 1)
+        run(Four{}, One{});
+      else
+        run(Four{}, Four{});
+    }
   }
-  k_join<T><<<static_cast<unsigned>(ceil_div(static_cast<uint64_t>(a.kv_heads) * a.all_rows, kWaves)), kThreads, 0, s>>>(a);
-  if (a.whole) {
-    const uint64_t key_blocks = static_cast<uint64_t>(a.batch) * a.kv_heads * ceil_div(a.capacity, 64);
-    k_weights<T, D, A><<<static_cast<unsigned>(key_blocks), kThreads, 0, s>>>(a);
+  // A workgroup per row where there are many ranges, else a wavefront.
+  const uint32_t tasks = a.kv_heads * a.all_rows;
+  const uint32_t fused = l.stored ? l.weight_blocks : 0;
+  if (a.prefix_splits + a.own_splits > 8) {
+    k_join<T, D, 4><<<tasks + fused, kThreads, 0, s>>>(a, tasks);
+  } else {
+    const uint32_t blocks_of_rows = static_cast<uint32_t>(ceil_div(tasks, kWaves));
+    k_join<T, D, 1><<<blocks_of_rows + fused, kThreads, 0, s>>>(a, blocks_of_rows);
   }
+  if (l.weighted && !l.stored) k_weights<T, D, A><<<l.weight_blocks, kThreads, 0, s>>>(a);
 }
 
 template <class T, int D>
@@ -710,7 +910,7 @@ void submit(dl_queue* queue, int dtype, const dl_batch_shape* shape, uint64_t pr
                         : static_cast<int>(l.args.width) == l.features ? Access::kWhole
                                                                        : Access::kPieces;
   if (access == Access::kElements) {  // the ranges, and with them the workspace, stay
-    l.set_tiles(1);
+    l.set_tiles(1, 1);
     l.count_blocks();
   }
   require(o.query && o.key && o.value && o.lengths && o.output && o.scale, "null operand");
@@ -718,7 +918,6 @@ void submit(dl_queue* queue, int dtype, const dl_batch_shape* shape, uint64_t pr
   require(!weighted || (o.weights && o.weights_out), "null weights");
   require(o.workspace != nullptr && reinterpret_cast<uintptr_t>(o.workspace) % 16 == 0, "workspace null or not 16-byte aligned");
   require(o.workspace_bytes >= l.bytes(), "workspace too small", DL_LENGTH_ERROR);
-  if (weighted) product({shape->batch, shape->kv_heads, ceil_div(shape->capacity, 64)}, 1u << 30, kTooMany);
   enter(queue);
   Args& a = l.args;
   a.query = o.query;
@@ -732,7 +931,8 @@ void submit(dl_queue* queue, int dtype, const dl_batch_shape* shape, uint64_t pr
   char* room = static_cast<char*>(o.workspace);
   a.part = reinterpret_cast<float2*>(room);
   a.sums = reinterpret_cast<float*>(room + l.part_bytes);
-  if (weighted) a.whole = reinterpret_cast<float2*>(room + l.part_bytes + l.sums_bytes);
+  a.whole = reinterpret_cast<float2*>(room + l.part_bytes + l.sums_bytes);
+  if (l.stored) a.scores = reinterpret_cast<float*>(room + l.part_bytes + l.sums_bytes + l.whole_bytes);
   a.weights = static_cast<const float*>(o.weights);
   a.weights_out = o.weights_out;
   if (dtype == DL_BF16)
