@@ -123,7 +123,7 @@ struct Operands<uint16_t, D, A> {
       load_words<T, 8, A>(base + 64 * s, offset, (4 * s + g) * 8, width, reinterpret_cast<uint32_t*>(&out[s]));
   }
   // The key of value row r in the order in which P holds them.
-  static __device__ __forceinline__ int value_key(int g, int r) { return (r / 4) * 16 + 4 * g + r % 4; }
+  static __device__ __forceinline__ constexpr int value_key(int g, int r) { return (r / 4) * 16 + 4 * g + r % 4; }
   // Scores of NQ row tiles against NK key tiles, the chains side by side.
   template <int NQ, int NK>
   static __device__ __forceinline__ void scores(const u32x4 (&k)[NK][kSteps], const u32x4 (&q)[NQ][kSteps], f32x4 (&s)[NQ][NK]) {
@@ -181,7 +181,7 @@ struct Operands<float, D, A> {
     for (int s = 0; s < kSteps; ++s)
       load_words<T, 4, A>(base + 64 * s, offset, (4 * s + g) * 4, width, reinterpret_cast<uint32_t*>(&out[s]));
   }
-  static __device__ __forceinline__ int value_key(int g, int r) { return 4 * g + r; }
+  static __device__ __forceinline__ constexpr int value_key(int g, int r) { return 4 * g + r; }
   template <int NQ, int NK>
   static __device__ __forceinline__ void scores(const u32x4 (&k)[NK][kSteps], const u32x4 (&q)[NQ][kSteps], f32x4 (&s)[NQ][NK]) {
 #pragma unroll
@@ -273,12 +273,6 @@ __device__ __forceinline__ void take_sign(float scale, u32x4 (&q)[N]) {
   }
 }
 
-// Wavefronts per SIMD that a kernel's registers are held to.
-template <class T, int D, int QT>
-constexpr int waves_per_simd() {
-  return D == 64 ? (QT == 1 ? 4 : QT == 2 ? 3 : 2) : D == 128 ? (QT == 4 ? 1 : 2) : 1;
-}
-
 // What a workgroup does: rows [first, first + count) of the batch's per KV head
 // against keys [begin, end) of one source, the result of range `slot`.
 struct Range {
@@ -288,16 +282,160 @@ struct Range {
   uint32_t least;             // keys that every row sees
 };
 
-template <class T, int D, int QT>
-struct Room {
-  static constexpr int C = D / 16;
-  f32x4 joined[QT == 1 ? 4 : 2 * QT][C][64];
-  float2 stats[2][QT][16];
-  float masked_p[kWaves][sizeof(T) == 2 ? 32 : 16][16];
+// One wavefront's 16 QT rows: running maximum, sum and output.
+template <class Ops, int QT>
+struct Rows {
+  static constexpr int C = Ops::C, kTiles = Ops::kTiles;
+  f32x4 o[QT][C];
+  float top[QT], sum[QT];
+  uint32_t limit[QT];  // keys that the lane's row sees
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      top[t] = -INFINITY;
+      sum[t] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < C; ++j) o[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+  // Scores of the step at key `at` to exponentials, everything so far rescaled
+  // where the maximum rises.  A score of a zero or NaN scale must not reach a
+  // hidden key either.
+  __device__ __forceinline__ void soften(f32x4 (&p)[QT][kTiles], bool masked, uint32_t at, float factor) {
+    const int g = threadIdx.x % 64 / 16;
+    auto hide = [&](float value) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (at + 16 * u + 4 * g + r >= limit[t]) p[t][u][r] = value;
+    };
+    if (masked) hide(-INFINITY);
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      float most = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kTiles; ++u) most = fmaxf(most, fmaxf(fmaxf(p[t][u][0], p[t][u][1]), fmaxf(p[t][u][2], p[t][u][3])));
+      if (__any(most * factor > top[t] + kSlack)) {
+        const float raised = fmaxf(top[t], group_max(most) * factor);
+        const float less = top[t] == -INFINITY ? 1.0f : exp2_of(top[t] - raised);  // nothing summed yet: zeros
+        top[t] = raised;
+        sum[t] = sum[t] * less;
+#pragma unroll
+        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * less;
+      }
+      const float from = -reference_of(top[t]);
+#pragma unroll
+      for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[t][u][r] = exp2_of(fma_rn(p[t][u][r], factor, from));
+    }
+    if (masked) hide(0.0f);
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int u = 0; u < kTiles; ++u) sum[t] = sum[t] + ((p[t][u][0] + p[t][u][1]) + (p[t][u][2] + p[t][u][3]));
+  }
+  // The values of a step with keys that some row does not see: cleared past
+  // the end.  An infinity or NaN in the others must not reach the rows that do
+  // not see it through 0 * inf, so such elements leave the product and are
+  // added to the rows that do.  `source` is the step's first row in memory.
+  __device__ __forceinline__ void hide_values(typename Ops::Values& v, const f32x4 (&p)[QT][kTiles], uint32_t at, uint32_t end,
+                                              const char* source, uint32_t stride, int width, float (*shares)[16]) {
+    using T = typename Ops::T;
+    const int lane = threadIdx.x % 64, i16 = lane % 16, g = lane / 16;
+    bool special = false;
+#pragma unroll
+    for (int r = 0; r < Ops::kValueRows; ++r)
+#pragma unroll
+      for (uint32_t& w : v.v[r]) {
+        if (at + Ops::value_key(g, r) >= end) w = 0;
+        const uint32_t plain = Ops::without_special(w);
+        special |= plain != w;
+        w = plain;
+      }
+    if (!__any(special)) return;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+#pragma unroll
+      for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) shares[16 * u + 4 * g + r][i16] = p[t][u][r];
+      __builtin_amdgcn_wave_barrier();
+      const uint32_t seen = min(min(limit[t], end), at + Ops::kKeys);
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        f32x4 to = o[t][j];
+#pragma unroll 1
+        for (uint32_t k = 0; at + k < seen; ++k) {
+          const T* row = reinterpret_cast<const T*>(source + k * stride);
+          const float share = shares[k][i16];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int f = (4 * g + r) * C + j;
+            const float x = f < width ? load_elem(row, f) : 0.0f;
+            to[r] = fabsf(x) < INFINITY ? to[r] : fma_rn(share, x, to[r]);
+          }
+        }
+        o[t][j] = to;
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  // Rows first + 16 t + lane % 16 of the range's result.  A lane holds features
+  // 4 C g .. of its row, 4 C of them in order.
+  __device__ __forceinline__ void store(const Args& a, const Range& range, uint32_t first, bool whole) const {
+    const int lane = threadIdx.x % 64, i16 = lane % 16, g = lane / 16;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      if (first + 16u * t + i16 >= range.count) continue;
+      const uint64_t row = (static_cast<uint64_t>(range.slot) * a.kv_heads + range.kvh) * a.all_rows + range.first + first + 16 * t + i16;
+      if (g == 0) a.part[row] = make_float2(top[t], sum[t]);
+      float* dst = a.sums + row * a.pitch;
+#pragma unroll
+      for (int m = 0; m < C; ++m) {
+        const uint32_t f = 4 * (g * C + m);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = o[t][(4 * m + e) % C][(4 * m + e) / C];
+        if (whole || f < a.pitch) *reinterpret_cast<f32x4*>(dst + f) = v;
+      }
+    }
+  }
 };
 
+// The operands of query rows first .. of the range's.
+template <class Ops, int QT>
+__device__ __forceinline__ void load_queries(const Args& a, const Range& range, uint32_t first, float scale,
+                                             u32x4 (&q)[QT][Ops::kSteps]) {
+  const int lane = threadIdx.x % 64, i16 = lane % 16, g = lane / 16;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const uint64_t at = query_offset(a, range.first + min(first + 16u * t + i16, range.count - 1), range.kvh);
+    Ops::load_row(reinterpret_cast<const char*>(static_cast<const typename Ops::T*>(a.query) + at), 16 * g, g, a.width, q[t]);
+    take_sign<Ops>(scale, q[t]);
+  }
+}
+
+// Few rows: every wavefront holds all of them and takes every fourth step, its
+// keys and values straight from memory, a step ahead.
+template <class Ops, int QT>
+struct Joined {
+  f32x4 o[2 * QT][Ops::C][64];
+};
+
+template <int Bytes>
+__device__ __forceinline__ uint8_t* joined_room() {
+  __shared__ __align__(16) uint8_t room[Bytes];
+  return room;
+}
+
 template <class T, int D, int QT, Access A>
-__device__ __forceinline__ void run_range(const Args& a, const Range& range, const uint32_t (&limit)[QT], Room<T, D, QT>& room) {
+__device__ __forceinline__ void run_apart(const Args& a, const Range& range, Rows<Operands<T, D, A>, QT>& rows,
+                                          Joined<Operands<T, D, A>, QT>& room, float (*shares)[16]) {
   using Ops = Operands<T, D, A>;
   constexpr int C = Ops::C, KT = Ops::kKeys, kTiles = Ops::kTiles;
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -305,24 +443,9 @@ __device__ __forceinline__ void run_range(const Args& a, const Range& range, con
   const int width = a.width;
   const uint32_t stride = a.kv_heads * a.width * sizeof(T), end = range.end;
   const float scale = *a.scale, factor = factor_of(scale);
-
   u32x4 q[QT][Ops::kSteps];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const uint64_t at = query_offset(a, range.first + min(16u * t + i16, range.count - 1), range.kvh);
-    Ops::load_row(reinterpret_cast<const char*>(static_cast<const T*>(a.query) + at), 16 * g, g, width, q[t]);
-    take_sign<Ops>(scale, q[t]);
-  }
-
-  f32x4 o[QT][C];
-  float top[QT], sum[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    top[t] = -INFINITY;
-    sum[t] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < C; ++j) o[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  load_queries<Ops>(a, range, 0, scale, q);
+  rows.clear();
 
   u32x4 kf[kTiles][Ops::kSteps];
   typename Ops::Values vf;
@@ -343,21 +466,6 @@ __device__ __forceinline__ void run_range(const Args& a, const Range& range, con
     for (int r = 0; r < Ops::kValueRows; ++r)
       load_words<T, C, A>(base, min(value_offset + Ops::value_key(0, r) * stride, most), i16 * C, width, vf.v[r]);
   };
-  // The elements of the step's first `seen` keys that are not finite, added to
-  // the lane's row of outputs in `joined`.
-  auto add_special = [&](const char* row, uint32_t seen) {
-    for (uint32_t k = 0; k < seen; ++k, row += stride) {
-      const float share = room.masked_p[wave][k][i16];
-#pragma unroll 1
-      for (int m = 0; m < 4 * C; ++m) {
-        const int f = 4 * g * C + m;
-        const float v = f < width ? load_elem(reinterpret_cast<const T*>(row), f) : 0.0f;
-        float& to = reinterpret_cast<float*>(&room.joined[wave][m % C][lane])[m / C];
-        if (!(fabsf(v) < INFINITY)) to = fma_rn(share, v, to);
-      }
-    }
-  };
-
   // Steps past the range repeat its last key: operands are defined on every
   // path.  (With the loads under a condition the compiler has reused part of
   // a loaded row's registers before its last use.)
@@ -371,150 +479,197 @@ __device__ __forceinline__ void run_range(const Args& a, const Range& range, con
     f32x4 p[QT][kTiles];
     Ops::scores(kf, q, p);
     load_keys(ahead);
-    if (range.scores) {
+    if (range.scores && static_cast<uint32_t>(i16) < range.count) {
       float* row = range.scores + static_cast<uint64_t>(i16) * a.score_pitch + at + 4 * g;
-      if (static_cast<uint32_t>(i16) < range.count) {
 #pragma unroll
-        for (int u = 0; u < kTiles; ++u) *reinterpret_cast<f32x4*>(row + 16 * u) = p[0][u];
-      }
+      for (int u = 0; u < kTiles; ++u) *reinterpret_cast<f32x4*>(row + 16 * u) = p[0][u];
     }
     const bool masked = at + KT > range.least;
-    if (masked) {
-#pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int u = 0; u < kTiles; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (at + 16 * u + 4 * g + r >= limit[t]) p[t][u][r] = -INFINITY;
-    }
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      float most = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < kTiles; ++u) most = fmaxf(most, fmaxf(fmaxf(p[t][u][0], p[t][u][1]), fmaxf(p[t][u][2], p[t][u][3])));
-      if (__any(most * factor > top[t] + kSlack)) {
-        const float raised = fmaxf(top[t], group_max(most) * factor);
-        const float less = top[t] == -INFINITY ? 1.0f : exp2_of(top[t] - raised);  // nothing summed yet: zeros
-        top[t] = raised;
-        sum[t] = sum[t] * less;
-#pragma unroll
-        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * less;
-      }
-      const float from = -reference_of(top[t]);
-#pragma unroll
-      for (int u = 0; u < kTiles; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) p[t][u][r] = exp2_of(fma_rn(p[t][u][r], factor, from));
-    }
-    if (masked) {
-      // A score of a zero or NaN scale must not reach a hidden key.  Values of
-      // keys past the end are cleared.  An infinity or NaN in the values of a
-      // key that only some rows see must not reach the others through 0 * inf:
-      // such elements leave the product and are added row by row.
-      bool special = false;
-#pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int u = 0; u < kTiles; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (at + 16 * u + 4 * g + r >= limit[t]) p[t][u][r] = 0.0f;
-#pragma unroll
-      for (int r = 0; r < Ops::kValueRows; ++r)
-#pragma unroll
-        for (uint32_t& w : vf.v[r]) {
-          if (at + Ops::value_key(g, r) >= end) w = 0;
-          const uint32_t plain = Ops::without_special(w);
-          special |= plain != w;
-          w = plain;
-        }
-      if (__any(special)) {
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-#pragma unroll
-          for (int u = 0; u < kTiles; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) room.masked_p[wave][16 * u + 4 * g + r][i16] = p[t][u][r];
-#pragma unroll
-          for (int j = 0; j < C; ++j) room.joined[wave][j][lane] = o[t][j];
-          __builtin_amdgcn_wave_barrier();
-          const uint32_t seen = min(min(limit[t], end), at + KT);
-          add_special(range.values + static_cast<uint64_t>(at) * stride, seen > at ? seen - at : 0);
-          __builtin_amdgcn_wave_barrier();
-#pragma unroll
-          for (int j = 0; j < C; ++j) o[t][j] = room.joined[wave][j][lane];
-        }
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < QT; ++t)
-#pragma unroll
-      for (int u = 0; u < kTiles; ++u) sum[t] = sum[t] + ((p[t][u][0] + p[t][u][1]) + (p[t][u][2] + p[t][u][3]));
-    Ops::template products<QT>(vf, p, o);
+    rows.soften(p, masked, at, factor);
+    if (masked)
+      rows.hide_values(vf, p, at, end, range.values + static_cast<uint64_t>(at) * stride, stride, width, shares + wave * 32);
+    Ops::template products<QT>(vf, p, rows.o);
     load_values(ahead);
     at = next;
   }
 #pragma unroll
-  for (int t = 0; t < QT; ++t) sum[t] = group_sum(sum[t]);
+  for (int t = 0; t < QT; ++t) rows.sum[t] = group_sum(rows.sum[t]);
 
   // Join the wavefronts: 2 and 3 into 0 and 1, then 1 into 0; those without a
-  // step have nothing to give.
+  // step have nothing to give.  A giver's maxima and sums lie in its own shares.
+  auto stats = [&](int of) { return reinterpret_cast<float2*>(shares + of * 32); };
   const uint32_t steps = end > range.begin ? (end - range.begin + KT - 1) / KT : 0;
-  __syncthreads();
 #pragma unroll
   for (int half = 2; half; half /= 2) {
     if (steps <= static_cast<uint32_t>(half)) continue;
     if (wave >= half && wave < 2 * half) {
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        if (g == 0) room.stats[wave - half][t][i16] = make_float2(top[t], sum[t]);
+        if (g == 0) stats(wave)[16 * t + i16] = make_float2(rows.top[t], rows.sum[t]);
 #pragma unroll
-        for (int j = 0; j < C; ++j) room.joined[(wave - half) * QT + t][j][lane] = o[t][j];
+        for (int j = 0; j < C; ++j) room.o[(wave - half) * QT + t][j][lane] = rows.o[t][j];
       }
     }
     __syncthreads();
     if (wave < half) {
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        const float2 other = room.stats[wave][t][i16];
-        const float raised = fmaxf(top[t], other.x), from = reference_of(raised);
-        const float mine = exp2_of(top[t] - from), theirs = exp2_of(other.x - from);
-        top[t] = raised;
-        sum[t] = fma_rn(sum[t], mine, other.y * theirs);
+        const float2 other = stats(wave + half)[16 * t + i16];
+        const float raised = fmaxf(rows.top[t], other.x), from = reference_of(raised);
+        const float mine = exp2_of(rows.top[t] - from), theirs = exp2_of(other.x - from);
+        rows.top[t] = raised;
+        rows.sum[t] = fma_rn(rows.sum[t], mine, other.y * theirs);
 #pragma unroll
-        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * mine + room.joined[wave * QT + t][j][lane] * theirs;
+        for (int j = 0; j < C; ++j) rows.o[t][j] = rows.o[t][j] * mine + room.o[wave * QT + t][j][lane] * theirs;
       }
     }
     __syncthreads();
   }
-  if (wave) return;
-  // A lane holds features 4 C g .. of its row, 4 C of them in order.
+  if (wave == 0) rows.store(a, range, 0, A == Access::kWhole);
+}
+
+// Many BF16 rows: a wavefront holds 16 QT rows of its own, and the four share
+// the keys and values through LDS, loaded there directly, a tile ahead.  A row
+// of a tile keeps its 16-byte pieces at piece ^ swizzle(row): the sixteen rows
+// of a key operand and the sixteen pieces of a value operand lie in distinct
+// banks.
+template <int D>
+struct Stage {
+  static constexpr int kKeys = D == 256 ? 32 : 64, kPieces = D / 8, kRowBytes = 2 * D;
+  static constexpr int kBytes = kKeys * kRowBytes;       // of keys, and of values
+  static constexpr int kLoads = kBytes / 1024 / kWaves;  // 1024-byte loads of a wavefront
+  static __device__ __forceinline__ uint32_t swizzle(uint32_t row) { return D == 64 ? row / 2 % 8 : row % 16; }
+};
+// A separate LDS object per stage, so that the compiler adds no waits between
+// the loads in flight and the reads.
+template <int D, int I>
+__device__ __forceinline__ uint8_t* stage_room() {
+  __shared__ __align__(1024) uint8_t room[2 * Stage<D>::kBytes];
+  return room;
+}
+
+template <int D, int QT, Access A>
+__device__ __forceinline__ void run_together(const Args& a, const Range& range, Rows<Operands<uint16_t, D, A>, QT>& rows,
+                                             float (*shares)[16]) {
+  using T = uint16_t;
+  using Ops = Operands<T, D, A>;
+  using S = Stage<D>;
+  constexpr int C = Ops::C, KT = Ops::kKeys, kTiles = Ops::kTiles;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t i16 = lane % 16, g = lane / 16;
+  const uint32_t width = a.width, stride = a.kv_heads * a.width * sizeof(T), end = range.end;
+  const float scale = *a.scale, factor = factor_of(scale);
+  const uint32_t first = wave * 16 * QT;
+  u32x4 q[QT][Ops::kSteps];
+  load_queries<Ops>(a, range, first, scale, q);
+  rows.clear();
+
+  auto issue = [&](uint8_t* room, uint32_t at) {
+    const char* keys = range.keys + static_cast<uint64_t>(at) * stride;
+    const char* values = range.values + static_cast<uint64_t>(at) * stride;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    if (16u * t + i16 >= range.count) continue;
-    const uint64_t row = (static_cast<uint64_t>(range.slot) * a.kv_heads + range.kvh) * a.all_rows + range.first + 16 * t + i16;
-    if (g == 0) a.part[row] = make_float2(top[t], sum[t]);
-    float* dst = a.sums + row * a.pitch;
-#pragma unroll
-    for (int m = 0; m < C; ++m) {
-      const uint32_t f = 4 * (g * C + m);
-      f32x4 v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = o[t][(4 * m + e) % C][(4 * m + e) / C];
-      if (A == Access::kWhole || f < a.pitch) *reinterpret_cast<f32x4*>(dst + f) = v;
+    for (int i = 0; i < S::kLoads; ++i) {
+      const uint32_t slot = (i * kWaves + wave) * 64 + lane, row = slot / S::kPieces;
+      uint32_t piece = slot % S::kPieces ^ S::swizzle(row);
+      if (A != Access::kWhole && piece * 8 >= width) piece = 0;  // not a piece of the row: cleared or not stored
+      const uint32_t offset = min(row, end - at - 1) * stride + piece * 16;
+      uint8_t* to = room + (i * kWaves + wave) * 1024;
+      __builtin_amdgcn_global_load_lds((const global_ptr*)(keys + offset), (lds_ptr*)to, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const global_ptr*)(values + offset), (lds_ptr*)(to + S::kBytes), 16, 0, 0);
     }
+  };
+  auto step = [&](const uint8_t* room, uint32_t row0, uint32_t at) {
+    u32x4 kf[kTiles][Ops::kSteps];
+#pragma unroll
+    for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+      for (int s = 0; s < Ops::kSteps; ++s) {
+        kf[u][s] = *reinterpret_cast<const u32x4*>(room + (row0 + 16 * u + i16) * S::kRowBytes + ((4 * s + g) ^ S::swizzle(i16)) * 16);
+        if (A != Access::kWhole && (4 * s + g) * 8 >= width) kf[u][s] = u32x4{};
+      }
+    f32x4 p[QT][kTiles];
+    Ops::scores(kf, q, p);
+    const bool masked = at + KT > range.least;
+    rows.soften(p, masked, at, factor);
+    typename Ops::Values vf;
+#pragma unroll
+    for (int r = 0; r < Ops::kValueRows; ++r) {
+      const uint32_t row = Ops::value_key(g, r);
+      const uint8_t* line = room + S::kBytes + (row0 + row) * S::kRowBytes;
+      if constexpr (C == 4) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(line + ((i16 / 2) ^ S::swizzle(row)) * 16 + i16 % 2 * 8);
+        vf.v[r][0] = v.x;
+        vf.v[r][1] = v.y;
+      } else {
+#pragma unroll
+        for (int m = 0; m < C / 8; ++m) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(line + ((i16 * (C / 8) + m) ^ S::swizzle(row)) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vf.v[r][4 * m + e] = v[e];
+        }
+      }
+    }
+    if (masked)
+      rows.hide_values(vf, p, at, end, range.values + static_cast<uint64_t>(at) * stride, stride, width, shares + wave * 32);
+    Ops::template products<QT>(vf, p, rows.o);
+  };
+  auto tile = [&](uint8_t* room, uint8_t* other, uint32_t at) {
+    __builtin_amdgcn_s_waitcnt(vm_wait(0));  // this tile has landed
+    __syncthreads();                         // for everybody, and the other buffer is read
+    if (at + S::kKeys < end) issue(other, at + S::kKeys);
+    __builtin_amdgcn_sched_barrier(0);
+    if (first >= range.count) return;
+#pragma unroll
+    for (int k = 0; k < S::kKeys; k += KT)
+      if (at + k < end) step(room, k, at + k);
+  };
+  if (range.begin < end) issue(stage_room<D, 0>(), range.begin);
+  for (uint32_t at = range.begin; at < end; at += 2 * S::kKeys) {
+    tile(stage_room<D, 0>(), stage_room<D, 1>(), at);
+    if (at + S::kKeys < end) tile(stage_room<D, 1>(), stage_room<D, 0>(), at + S::kKeys);
+  }
+#pragma unroll
+  for (int t = 0; t < QT; ++t) rows.sum[t] = group_sum(rows.sum[t]);
+  if (first < range.count) rows.store(a, range, first, A == Access::kWhole);
+}
+
+// Rows of a workgroup against one source: kApart1 and kApart2 hold 16 and 32 in
+// every wavefront, kTogether1 and kTogether2 16 and 32 in each.
+enum class Mode { kApart1, kApart2, kTogether1, kTogether2 };
+constexpr bool together(Mode m) { return m == Mode::kTogether1 || m == Mode::kTogether2; }
+constexpr int tiles_of(Mode m) { return m == Mode::kApart1 || m == Mode::kTogether1 ? 1 : 2; }
+constexpr uint32_t rows_of(Mode m) { return 16 * tiles_of(m) * (together(m) ? kWaves : 1); }
+
+// Wavefronts per SIMD that the registers are held to.
+template <int D, Mode M>
+constexpr int waves_per_simd() {
+  return D == 256 ? 1 : D == 64 && tiles_of(M) == 1 ? 3 : 2;
+}
+
+template <class T, int D, Mode M, Access A, Mode Kernel, class Limit>
+__device__ __forceinline__ void run_range(const Args& a, const Range& range, float (*shares)[16], Limit&& limit) {
+  using Ops = Operands<T, D, A>;
+  constexpr int QT = tiles_of(M);
+  Rows<Ops, QT> rows;
+  const uint32_t first = together(M) ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 16 * QT : 0;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) rows.limit[t] = limit(min(first + 16 * t + threadIdx.x % 16, range.count - 1));
+  if constexpr (together(M)) {
+    run_together<D, QT, A>(a, range, rows, shares);
+  } else if constexpr (together(Kernel)) {  // the stages are free: no block runs both
+    static_assert(sizeof(Joined<Ops, QT>) <= 2 * Stage<D>::kBytes, "joined outputs outgrow a stage");
+    run_apart<T, D, QT, A>(a, range, rows, *reinterpret_cast<Joined<Ops, QT>*>(stage_room<D, 0>()), shares);
+  } else {
+    run_apart<T, D, QT, A>(a, range, rows, *reinterpret_cast<Joined<Ops, QT>*>(joined_room<sizeof(Joined<Ops, tiles_of(Kernel)>)>()), shares);
   }
 }
 
-// QP row tiles per workgroup against the prefix, QO against an own cache: a
-// sequence of a decode step has few rows where the batch has many.
-template <class T, int D, int QP, int QO, Access A>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(waves_per_simd<T, D, QP>())))
+// Mode P against the prefix, O against an own cache: a sequence of a decode
+// step has few rows where the batch has many.
+template <class T, int D, Mode P, Mode O, Access A>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(waves_per_simd<D, P>())))
 void k_ranges(const Args a) {
-  __shared__ __align__(16) Room<T, D, QP> room;
-  const int i16 = threadIdx.x % 16;
-  const uint64_t stride = static_cast<uint64_t>(a.kv_heads) * a.width;
+  __shared__ float shares[kWaves * 32][16];
   Range range;
   uint32_t group, tile;
   if (blockIdx.x < a.prefix_blocks) {
@@ -525,16 +680,13 @@ void k_ranges(const Args a) {
     range.begin = range.slot * each;
     if (range.begin >= a.prefix) return;
     range.end = range.least = min(range.begin + each, a.prefix);
-    range.first = tile * 16 * QP;
-    range.count = min(a.all_rows - range.first, 16u * QP);
+    range.first = tile * rows_of(P);
+    range.count = min(a.all_rows - range.first, rows_of(P));
     range.scores = nullptr;
     const uint64_t at = static_cast<uint64_t>(range.kvh) * a.width * sizeof(T);
     range.keys = static_cast<const char*>(a.prefix_key) + at;
     range.values = static_cast<const char*>(a.prefix_value) + at;
-    uint32_t limit[QP];
-#pragma unroll
-    for (int t = 0; t < QP; ++t) limit[t] = range.end;
-    run_range<T, D, QP, A>(a, range, limit, room);
+    run_range<T, D, P, A, P>(a, range, shares, [&](uint32_t) { return range.end; });
     return;
   }
   if (!block_task(blockIdx.x - a.prefix_blocks, a.batch * a.kv_heads * a.own_splits, a.own_tiles, group, tile)) return;
@@ -544,20 +696,19 @@ void k_ranges(const Args a) {
   const uint32_t n = length_of(a, b), each = range_keys(n, a.own_splits);
   range.begin = split * each;
   if (range.begin >= n) return;
-  const uint32_t first = tile * 16 * QO;
-  range.count = min(a.seq_rows - first, 16u * QO);
+  const uint32_t first = tile * rows_of(O);
+  auto limit = [&](uint32_t row) { return visible(n, a.rows, (first + row) / a.group); };
+  range.count = min(a.seq_rows - first, rows_of(O));
   range.end = min(range.begin + each, n);
-  range.least = min(range.end, visible(n, a.rows, first / a.group));
-  range.end = min(range.end, max(range.begin, visible(n, a.rows, (first + range.count - 1) / a.group)));  // no row sees further
-  uint32_t limit[QO];
-#pragma unroll
-  for (int t = 0; t < QO; ++t) limit[t] = visible(n, a.rows, min(first + 16 * t + i16, first + range.count - 1) / a.group);
+  range.least = min(range.end, limit(0));
+  range.end = min(range.end, max(range.begin, limit(range.count - 1)));  // no row sees further
   range.first = b * a.seq_rows + first;
   range.scores = a.scores ? a.scores + ((static_cast<uint64_t>(b) * a.kv_heads + range.kvh) * a.seq_rows + first) * a.score_pitch : nullptr;
+  const uint64_t stride = static_cast<uint64_t>(a.kv_heads) * a.width;
   const uint64_t at = (b * a.capacity * stride + static_cast<uint64_t>(range.kvh) * a.width) * sizeof(T);
   range.keys = static_cast<const char*>(a.key) + at;
   range.values = static_cast<const char*>(a.value) + at;
-  run_range<T, D, QO, A>(a, range, limit, reinterpret_cast<Room<T, D, QO>&>(room));
+  run_range<T, D, O, A, P>(a, range, shares, limit);
 }
 
 // The ranges that hold something of one row, in order.
@@ -760,19 +911,21 @@ uint64_t product(std::initializer_list<uint64_t> factors, uint64_t most, const c
 // Row tiles per workgroup, ranges and workspace of one call.
 struct Layout {
   Args args{};
-  int prefix_q = 1, own_q = 1;  // row tiles of 16
+  Mode prefix_mode = Mode::kApart1, own_mode = Mode::kApart1;
   int features = 64;            // D
   bool weighted = false, stored = false;
   uint64_t part_bytes = 0, sums_bytes = 0, whole_bytes = 0, score_bytes = 0;
   uint32_t own_blocks = 0, weight_blocks = 0;
 
   uint64_t bytes() const { return part_bytes + sums_bytes + whole_bytes + score_bytes; }
-  void set_tiles(int prefix, int own) {
-    prefix_q = prefix;
-    own_q = own;
-    args.prefix_tiles = static_cast<uint32_t>(ceil_div(args.all_rows, 16 * prefix));
-    args.own_tiles = static_cast<uint32_t>(ceil_div(args.seq_rows, 16 * own));
+  void set_modes(Mode prefix, Mode own) {
+    prefix_mode = prefix;
+    own_mode = own;
+    args.prefix_tiles = static_cast<uint32_t>(ceil_div(args.all_rows, rows_of(prefix)));
+    args.own_tiles = static_cast<uint32_t>(ceil_div(args.seq_rows, rows_of(own)));
   }
+  // 32 rows where D = 256 has registers for 16.
+  Mode apart(uint32_t rows) const { return rows <= 16 || features == 256 ? Mode::kApart1 : Mode::kApart2; }
   void count_blocks() {
     auto blocks = [&](std::initializer_list<uint64_t> groups, uint64_t tiles) {
       const uint64_t rounded = ceil_div(product(groups, kMostBlocks, kTooMany), 8) * 8;
@@ -807,13 +960,17 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted) {
   l.features = a.width <= 64 ? 64 : a.width <= 128 ? 128 : 256;
   l.weighted = weighted;
   l.stored = weighted && a.seq_rows <= 16;
-  // Rows per workgroup: as many tiles as the rows fill; D = 256 has registers
-  // for two.
-  auto tiles = [&](uint32_t rows) { return rows <= 16 ? 1 : rows <= 32 || l.features == 256 ? 2 : 4; };
-  const int own = tiles(a.seq_rows), all = prefix ? tiles(a.all_rows) : own;
-  l.set_tiles(all, own == 1 ? 1 : all);
+  // Few rows: every wavefront has them all.  More: 64, or where that still
+  // fills the chip 128, a workgroup.
+  auto mode_of = [&](uint32_t rows, uint64_t groups) {
+    if (rows <= 32) return l.apart(rows);
+    return l.features < 256 && ceil_div(rows, 128) * groups >= 512 ? Mode::kTogether2 : Mode::kTogether1;
+  };
+  const Mode own = mode_of(a.seq_rows, uint64_t{a.batch} * a.kv_heads * ceil_div(a.capacity, kRound));
+  const Mode all = prefix ? mode_of(a.all_rows, a.kv_heads * ceil_div(prefix, kRound)) : own;
+  l.set_modes(all, a.seq_rows <= 16 ? Mode::kApart1 : all);
   // Ranges: as many workgroups as the chip holds at once, each with whole rounds of keys.
-  const uint64_t held = 256 * (l.features == 64 ? (all == 1 ? 4 : all == 2 ? 3 : 2) : l.features == 128 && all < 4 ? 2 : 1);
+  const uint64_t held = 256 * (l.features == 256 ? 1 : l.features == 64 && tiles_of(all) == 1 ? 3 : 2);
   const double work = static_cast<double>(a.kv_heads) *
                       (static_cast<double>(a.prefix_tiles) * a.prefix +
                        static_cast<double>(a.batch) * a.own_tiles * a.capacity);
@@ -838,25 +995,26 @@ template <class T, int D, Access A>
 void launch(hipStream_t s, const Layout& l) {
   const Args& a = l.args;
   const unsigned blocks = a.prefix_blocks + l.own_blocks;  // at most 2^31
-  auto run = [&](auto prefix_q, auto own_q) {
-    k_ranges<T, D, decltype(prefix_q)::value, decltype(own_q)::value, A><<<blocks, kThreads, 0, s>>>(a);
+  auto run = [&](auto prefix, auto own) {
+    k_ranges<T, D, decltype(prefix)::value, decltype(own)::value, A><<<blocks, kThreads, 0, s>>>(a);
   };
-  using One = std::integral_constant<int, 1>;
-  using Two = std::integral_constant<int, 2>;
-  using Four = std::integral_constant<int, 4>;
-  if (l.prefix_q == 1) {
-    run(One{}, One{});
+  auto run_own = [&](auto prefix) {
+    if (l.own_mode == Mode::kApart1)
+      run(prefix, std::integral_constant<Mode, Mode::kApart1>{});
+    else
+      run(prefix, prefix);
+  };
+  if (l.prefix_mode == Mode::kApart1) {
+    run(std::integral_constant<Mode, Mode::kApart1>{}, std::integral_constant<Mode, Mode::kApart1>{});
   } else if constexpr (A != Access::kElements) {
-    if (l.prefix_q == 2) {
-      if (l.own_q == 1)
-        run(Two{}, One{});
-      else
-        run(Two{}, Two{});
-    } else if constexpr (D != 256) {
-      if (l.own_q == 1)
-        run(Four{}, One{});
-      else
-        run(Four{}, Four{});
+    if constexpr (D != 256) {
+      if (l.prefix_mode == Mode::kApart2) run_own(std::integral_constant<Mode, Mode::kApart2>{});
+    }
+    if constexpr (std::is_same_v<T, uint16_t>) {
+      if (l.prefix_mode == Mode::kTogether1) run_own(std::integral_constant<Mode, Mode::kTogether1>{});
+      if constexpr (D != 256) {
+        if (l.prefix_mode == Mode::kTogether2) run_own(std::integral_constant<Mode, Mode::kTogether2>{});
+      }
     }
   }
   // A workgroup per row where there are many ranges, else a wavefront.
@@ -909,8 +1067,11 @@ void submit(dl_queue* queue, int dtype, const dl_batch_shape* shape, uint64_t pr
   const Access access = !pieces ? Access::kElements
                         : static_cast<int>(l.args.width) == l.features ? Access::kWhole
                                                                        : Access::kPieces;
-  if (access == Access::kElements) {  // the ranges, and with them the workspace, stay
-    l.set_tiles(1, 1);
+  // The shared tiles are 16-byte pieces of BF16.  FP32 rows and others run
+  // apart; the ranges, and with them the workspace, stay.
+  if (access == Access::kElements || (dtype == DL_F32 && together(l.prefix_mode))) {
+    const Mode mode = access == Access::kElements ? Mode::kApart1 : l.apart(32);
+    l.set_modes(mode, l.own_mode == Mode::kApart1 ? Mode::kApart1 : mode);
     l.count_blocks();
   }
   require(o.query && o.key && o.value && o.lengths && o.output && o.scale, "null operand");
