@@ -41,10 +41,10 @@ namespace {
 constexpr int kThreads = 256, kWaves = 4;
 constexpr float kLog2e = 0x1.715476p+0f;
 // Scores are in units of ln 2 from the first maximum on: exponentials are the
-// hardware's exp2 of one fused multiply-add.  A maximum is raised only when a
-// score passes it by kSlack: exponentials stay below 2^12, and most steps
-// rescale nothing.
-constexpr float kSlack = 12.0f;
+// hardware's exp2 of one fused multiply-add.  A maximum is raised only when the
+// exponentials of a lane's keys of one step sum to more than kMostSum: most
+// steps rescale nothing.
+constexpr float kMostSum = 8192.0f;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -93,6 +93,10 @@ __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2
 // The value subtracted from scores: 0 while no score is finite, so that
 // exp2(-inf - m) is 0 and not NaN.
 __device__ __forceinline__ float reference_of(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// Code that few steps run is laid out behind the rest: a workgroup's first pass
+// through a step is bound by instruction fetch.
+__device__ __forceinline__ bool rare(bool condition) { return __builtin_expect(condition, false); }
 
 __device__ __forceinline__ float group_max(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -147,12 +151,16 @@ struct Operands<uint16_t, D, A> {
     return __builtin_bit_cast(bf16x8, w);
   }
   template <int QT>
-  static __device__ __forceinline__ void products(const Values& v, const f32x4 (&p)[QT][kTiles], f32x4 (&o)[QT][C]) {
-    bf16x8 b[QT];
+  static __device__ __forceinline__ void rounded(const f32x4 (&p)[QT][kTiles], bf16x8 (&b)[QT]) {
 #pragma unroll
     for (int t = 0; t < QT; ++t)
 #pragma unroll
       for (int e = 0; e < 8; ++e) b[t][e] = static_cast<__bf16>(p[t][e / 4][e % 4]);
+  }
+  template <int QT>
+  static __device__ __forceinline__ void products(const Values& v, const f32x4 (&p)[QT][kTiles], f32x4 (&o)[QT][C]) {
+    bf16x8 b[QT];
+    rounded<QT>(p, b);
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const bf16x8 a = value_tile(v, j);
@@ -218,10 +226,6 @@ __host__ __device__ inline uint32_t range_keys(uint32_t keys, uint32_t splits) {
   const uint32_t each = keys / splits + (keys % splits != 0);
   return (each + kRound - 1) / kRound * kRound;
 }
-__host__ __device__ inline uint32_t ranges_of(uint32_t keys, uint32_t splits) {
-  const uint32_t each = range_keys(keys, splits);
-  return keys ? keys / each + (keys % each != 0) : 0;
-}
 
 struct Args {
   const void *query, *prefix_key, *prefix_value, *key, *value;
@@ -236,7 +240,8 @@ struct Args {
   float* weights_out;
   uint32_t batch, rows, q_heads, kv_heads, group, width, prefix, capacity;
   uint32_t seq_rows, all_rows;          // rows of one sequence and of the batch, per KV head
-  uint32_t prefix_splits, own_splits;   // most ranges of a source
+  uint32_t prefix_splits, own_splits;   // ranges of the prefix, most ranges of an own cache
+  uint32_t prefix_each;                 // keys of a range of the prefix
   uint32_t prefix_blocks, prefix_tiles, own_tiles;
   uint32_t pitch, score_pitch;          // row widths of `sums` and `scores`
 };
@@ -282,82 +287,84 @@ struct Range {
   uint32_t least;             // keys that every row sees
 };
 
-// One wavefront's 16 QT rows: running maximum, sum and output.
-template <class Ops, int QT>
+// One wavefront's 16 QT rows: running maximum, sum and output.  Lane 16 g + i
+// holds row i's scores of the keys 4 g + r of a step's tiles, and in o[t][j][r]
+// its feature (4 g + r) C + j, or 16 j + 4 g + r where value operands are read
+// across the rows of LDS (Across).
+template <class Ops, int QT, bool Across>
 struct Rows {
   static constexpr int C = Ops::C, kTiles = Ops::kTiles;
   f32x4 o[QT][C];
   float top[QT], sum[QT];
-  uint32_t limit[QT];  // keys that the lane's row sees
+  float from[QT], most[QT];  // added to scores; the largest step sum that raises nothing
+  uint32_t limit[QT];        // keys that the lane's row sees
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       top[t] = -INFINITY;
-      sum[t] = 0.0f;
+      from[t] = sum[t] = 0.0f;
+      most[t] = -1.0f;
 #pragma unroll
       for (int j = 0; j < C; ++j) o[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
   }
-  // Scores of the step at key `at` to exponentials, everything so far rescaled
-  // where the maximum rises.  A score of a zero or NaN scale must not reach a
-  // hidden key either.
+  static __device__ __forceinline__ int feature(int g, int j, int r) { return Across ? 16 * j + 4 * g + r : (4 * g + r) * C + j; }
+
+  // Scores of the step at key `at` to exponentials against the maximum so far.
+  // A step whose exponentials sum to more than 2^13 in some lane (its scores
+  // pass that maximum by as much), and the first, raise the maximum and rescale
+  // what is summed; the others need no maximum of their own.
   __device__ __forceinline__ void soften(f32x4 (&p)[QT][kTiles], bool masked, uint32_t at, float factor) {
     const int g = threadIdx.x % 64 / 16;
-    auto hide = [&](float value) {
 #pragma unroll
-      for (int t = 0; t < QT; ++t)
+    for (int t = 0; t < QT; ++t) {
+      auto hide = [&](f32x4 (&v)[kTiles], float value) {
 #pragma unroll
         for (int u = 0; u < kTiles; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (at + 16 * u + 4 * g + r >= limit[t]) p[t][u][r] = value;
-    };
-    if (masked) hide(-INFINITY);
+            if (at + 16 * u + 4 * g + r >= limit[t]) v[u][r] = value;
+      };
+      f32x4 e[kTiles];
+      auto weigh = [&] {
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      float most = -INFINITY;
+        for (int u = 0; u < kTiles; ++u)
 #pragma unroll
-      for (int u = 0; u < kTiles; ++u) most = fmaxf(most, fmaxf(fmaxf(p[t][u][0], p[t][u][1]), fmaxf(p[t][u][2], p[t][u][3])));
-      if (__any(most * factor > top[t] + kSlack)) {
-        const float raised = fmaxf(top[t], group_max(most) * factor);
+          for (int r = 0; r < 4; ++r) e[u][r] = exp2_of(fma_rn(p[t][u][r], factor, from[t]));
+        if (rare(masked)) hide(e, 0.0f);  // also the NaN of a hidden key under a zero scale
+        float s = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u) s = s + ((e[u][0] + e[u][1]) + (e[u][2] + e[u][3]));
+        return s;
+      };
+      float s = weigh();
+      if (rare(__any(!(s <= most[t])))) {
+        if (masked) hide(p[t], -INFINITY);
+        float high = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u) high = fmaxf(high, fmaxf(fmaxf(p[t][u][0], p[t][u][1]), fmaxf(p[t][u][2], p[t][u][3])));
+        const float raised = fmaxf(top[t], group_max(high) * factor);
         const float less = top[t] == -INFINITY ? 1.0f : exp2_of(top[t] - raised);  // nothing summed yet: zeros
         top[t] = raised;
+        from[t] = -reference_of(raised);
+        most[t] = raised == -INFINITY ? -1.0f : kMostSum;
         sum[t] = sum[t] * less;
 #pragma unroll
         for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * less;
+        s = weigh();
       }
-      const float from = -reference_of(top[t]);
+      sum[t] = sum[t] + s;
 #pragma unroll
-      for (int u = 0; u < kTiles; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) p[t][u][r] = exp2_of(fma_rn(p[t][u][r], factor, from));
+      for (int u = 0; u < kTiles; ++u) p[t][u] = e[u];
     }
-    if (masked) hide(0.0f);
-#pragma unroll
-    for (int t = 0; t < QT; ++t)
-#pragma unroll
-      for (int u = 0; u < kTiles; ++u) sum[t] = sum[t] + ((p[t][u][0] + p[t][u][1]) + (p[t][u][2] + p[t][u][3]));
   }
-  // The values of a step with keys that some row does not see: cleared past
-  // the end.  An infinity or NaN in the others must not reach the rows that do
-  // not see it through 0 * inf, so such elements leave the product and are
-  // added to the rows that do.  `source` is the step's first row in memory.
-  __device__ __forceinline__ void hide_values(typename Ops::Values& v, const f32x4 (&p)[QT][kTiles], uint32_t at, uint32_t end,
-                                              const char* source, uint32_t stride, int width, float (*shares)[16]) {
+  // Elements of a step's values that are not finite have left the product: they
+  // are added to the rows that see them.  `source` is the step's first row.
+  __device__ __forceinline__ void add_special(const f32x4 (&p)[QT][kTiles], uint32_t at, uint32_t end, const char* source,
+                                              uint32_t stride, int width, float (*shares)[16]) {
     using T = typename Ops::T;
     const int lane = threadIdx.x % 64, i16 = lane % 16, g = lane / 16;
-    bool special = false;
-#pragma unroll
-    for (int r = 0; r < Ops::kValueRows; ++r)
-#pragma unroll
-      for (uint32_t& w : v.v[r]) {
-        if (at + Ops::value_key(g, r) >= end) w = 0;
-        const uint32_t plain = Ops::without_special(w);
-        special |= plain != w;
-        w = plain;
-      }
-    if (!__any(special)) return;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
 #pragma unroll
@@ -375,7 +382,7 @@ struct Rows {
           const float share = shares[k][i16];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int f = (4 * g + r) * C + j;
+            const int f = feature(g, j, r);
             const float x = f < width ? load_elem(row, f) : 0.0f;
             to[r] = fabsf(x) < INFINITY ? to[r] : fma_rn(share, x, to[r]);
           }
@@ -385,8 +392,7 @@ struct Rows {
       __builtin_amdgcn_wave_barrier();
     }
   }
-  // Rows first + 16 t + lane % 16 of the range's result.  A lane holds features
-  // 4 C g .. of its row, 4 C of them in order.
+  // Rows first + 16 t + lane % 16 of the range's result.
   __device__ __forceinline__ void store(const Args& a, const Range& range, uint32_t first, bool whole) const {
     const int lane = threadIdx.x % 64, i16 = lane % 16, g = lane / 16;
 #pragma unroll
@@ -396,11 +402,13 @@ struct Rows {
       if (g == 0) a.part[row] = make_float2(top[t], sum[t]);
       float* dst = a.sums + row * a.pitch;
 #pragma unroll
-      for (int m = 0; m < C; ++m) {
-        const uint32_t f = 4 * (g * C + m);
-        f32x4 v;
+      for (int m = 0; m < C; ++m) {  // four features in order
+        const uint32_t f = Across ? 16 * m + 4 * g : 4 * (g * C + m);
+        f32x4 v = o[t][m];
+        if constexpr (!Across) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = o[t][(4 * m + e) % C][(4 * m + e) / C];
+          for (int e = 0; e < 4; ++e) v[e] = o[t][(4 * m + e) % C][(4 * m + e) / C];
+        }
         if (whole || f < a.pitch) *reinterpret_cast<f32x4*>(dst + f) = v;
       }
     }
@@ -434,7 +442,7 @@ __device__ __forceinline__ uint8_t* joined_room() {
 }
 
 template <class T, int D, int QT, Access A>
-__device__ __forceinline__ void run_apart(const Args& a, const Range& range, Rows<Operands<T, D, A>, QT>& rows,
+__device__ __forceinline__ void run_apart(const Args& a, const Range& range, Rows<Operands<T, D, A>, QT, false>& rows,
                                           Joined<Operands<T, D, A>, QT>& room, float (*shares)[16]) {
   using Ops = Operands<T, D, A>;
   constexpr int C = Ops::C, KT = Ops::kKeys, kTiles = Ops::kTiles;
@@ -486,8 +494,23 @@ __device__ __forceinline__ void run_apart(const Args& a, const Range& range, Row
     }
     const bool masked = at + KT > range.least;
     rows.soften(p, masked, at, factor);
-    if (masked)
-      rows.hide_values(vf, p, at, end, range.values + static_cast<uint64_t>(at) * stride, stride, width, shares + wave * 32);
+    if (rare(masked)) {
+      // Values of keys past the end are cleared.  An infinity or NaN in the
+      // values of a key that only some rows see must not reach the others
+      // through 0 * inf.
+      bool special = false;
+#pragma unroll
+      for (int r = 0; r < Ops::kValueRows; ++r)
+#pragma unroll
+        for (uint32_t& w : vf.v[r]) {
+          if (at + Ops::value_key(g, r) >= end) w = 0;
+          const uint32_t plain = Ops::without_special(w);
+          special |= plain != w;
+          w = plain;
+        }
+      if (rare(__any(special)))
+        rows.add_special(p, at, end, range.values + static_cast<uint64_t>(at) * stride, stride, width, shares + wave * 32);
+    }
     Ops::template products<QT>(vf, p, rows.o);
     load_values(ahead);
     at = next;
@@ -529,16 +552,20 @@ __device__ __forceinline__ void run_apart(const Args& a, const Range& range, Row
 }
 
 // Many BF16 rows: a wavefront holds 16 QT rows of its own, and the four share
-// the keys and values through LDS, loaded there directly, a tile ahead.  A row
-// of a tile keeps its 16-byte pieces at piece ^ swizzle(row): the sixteen rows
-// of a key operand and the sixteen pieces of a value operand lie in distinct
-// banks.
+// the keys and values through LDS, loaded there directly, a tile ahead.  Value
+// operands are read across the rows (a lane gives four features of one key and
+// gets one feature of four keys), so no register is permuted.  A row of a tile
+// keeps its 16-byte pieces at piece ^ swizzle(row): the sixteen rows of a key
+// operand, and the eight rows of two pieces that half a wavefront reads of a
+// value operand, lie in distinct banks.
 template <int D>
 struct Stage {
   static constexpr int kKeys = D == 256 ? 32 : 64, kPieces = D / 8, kRowBytes = 2 * D;
   static constexpr int kBytes = kKeys * kRowBytes;       // of keys, and of values
   static constexpr int kLoads = kBytes / 1024 / kWaves;  // 1024-byte loads of a wavefront
-  static __device__ __forceinline__ uint32_t swizzle(uint32_t row) { return D == 64 ? row / 2 % 8 : row % 16; }
+  static __device__ __forceinline__ uint32_t swizzle(uint32_t row) {
+    return D == 64 ? 2 * (row / 2 % 4) + row / 8 % 2 : 2 * (row % 8) + row / 8 % 2;
+  }
 };
 // A separate LDS object per stage, so that the compiler adds no waits between
 // the loads in flight and the reads.
@@ -548,8 +575,11 @@ __device__ __forceinline__ uint8_t* stage_room() {
   return room;
 }
 
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+
 template <int D, int QT, Access A>
-__device__ __forceinline__ void run_together(const Args& a, const Range& range, Rows<Operands<uint16_t, D, A>, QT>& rows,
+__device__ __forceinline__ void run_together(const Args& a, const Range& range, Rows<Operands<uint16_t, D, A>, QT, true>& rows,
                                              float (*shares)[16]) {
   using T = uint16_t;
   using Ops = Operands<T, D, A>;
@@ -578,7 +608,8 @@ __device__ __forceinline__ void run_together(const Args& a, const Range& range, 
       __builtin_amdgcn_global_load_lds((const global_ptr*)(values + offset), (lds_ptr*)(to + S::kBytes), 16, 0, 0);
     }
   };
-  auto step = [&](const uint8_t* room, uint32_t row0, uint32_t at) {
+  const uint32_t value_row = 4 * g + i16 / 4;  // the row of the lane's share of a value read
+  auto step = [&](uint8_t* room, uint32_t row0, uint32_t at) {
     u32x4 kf[kTiles][Ops::kSteps];
 #pragma unroll
     for (int u = 0; u < kTiles; ++u)
@@ -591,27 +622,41 @@ __device__ __forceinline__ void run_together(const Args& a, const Range& range, 
     Ops::scores(kf, q, p);
     const bool masked = at + KT > range.least;
     rows.soften(p, masked, at, factor);
-    typename Ops::Values vf;
+    // Feature 16 j + i16 of keys 16 u + 4 g ..: words 2 u, 2 u + 1.
+    u32x4 vf[C];
 #pragma unroll
-    for (int r = 0; r < Ops::kValueRows; ++r) {
-      const uint32_t row = Ops::value_key(g, r);
-      const uint8_t* line = room + S::kBytes + (row0 + row) * S::kRowBytes;
-      if constexpr (C == 4) {
-        const u32x2 v = *reinterpret_cast<const u32x2*>(line + ((i16 / 2) ^ S::swizzle(row)) * 16 + i16 % 2 * 8);
-        vf.v[r][0] = v.x;
-        vf.v[r][1] = v.y;
-      } else {
+    for (int j = 0; j < C; ++j)
 #pragma unroll
-        for (int m = 0; m < C / 8; ++m) {
-          const u32x4 v = *reinterpret_cast<const u32x4*>(line + ((i16 * (C / 8) + m) ^ S::swizzle(row)) * 16);
+      for (int u = 0; u < kTiles; ++u) {
+        uint8_t* from = room + S::kBytes + (row0 + 16 * u + value_row) * S::kRowBytes +
+                        ((2 * j + i16 / 2 % 2) ^ S::swizzle(value_row)) * 16 + i16 % 2 * 8;
+        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)from));
+        vf[j][2 * u] = v.x;
+        vf[j][2 * u + 1] = v.y;
+      }
+    if (rare(masked)) {  // as for rows apart
+      bool special = false;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) vf.v[r][4 * m + e] = v[e];
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t key = at + 16 * (w / 2) + 4 * g + 2 * (w % 2);
+        const uint32_t real = (key < end ? 0xffffu : 0u) | (key + 1 < end ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          const uint32_t word = vf[j][w] & real, plain = Ops::without_special(word);
+          special |= plain != word;
+          vf[j][w] = plain;
         }
       }
+      if (rare(__any(special)))
+        rows.add_special(p, at, end, range.values + static_cast<uint64_t>(at) * stride, stride, width, shares + wave * 32);
     }
-    if (masked)
-      rows.hide_values(vf, p, at, end, range.values + static_cast<uint64_t>(at) * stride, stride, width, shares + wave * 32);
-    Ops::template products<QT>(vf, p, rows.o);
+    bf16x8 b[QT];
+    Ops::template rounded<QT>(p, b);
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+        rows.o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[j]), b[t], rows.o[t][j], 0, 0, 0);
   };
   auto tile = [&](uint8_t* room, uint8_t* other, uint32_t at) {
     __builtin_amdgcn_s_waitcnt(vm_wait(0));  // this tile has landed
@@ -619,9 +664,8 @@ __device__ __forceinline__ void run_together(const Args& a, const Range& range, 
     if (at + S::kKeys < end) issue(other, at + S::kKeys);
     __builtin_amdgcn_sched_barrier(0);
     if (first >= range.count) return;
-#pragma unroll
-    for (int k = 0; k < S::kKeys; k += KT)
-      if (at + k < end) step(room, k, at + k);
+#pragma unroll 1
+    for (uint32_t k = 0; k < S::kKeys && at + k < end; k += KT) step(room, k, at + k);
   };
   if (range.begin < end) issue(stage_room<D, 0>(), range.begin);
   for (uint32_t at = range.begin; at < end; at += 2 * S::kKeys) {
@@ -633,11 +677,11 @@ __device__ __forceinline__ void run_together(const Args& a, const Range& range, 
   if (first < range.count) rows.store(a, range, first, A == Access::kWhole);
 }
 
-// Rows of a workgroup against one source: kApart1 and kApart2 hold 16 and 32 in
-// every wavefront, kTogether1 and kTogether2 16 and 32 in each.
-enum class Mode { kApart1, kApart2, kTogether1, kTogether2 };
-constexpr bool together(Mode m) { return m == Mode::kTogether1 || m == Mode::kTogether2; }
-constexpr int tiles_of(Mode m) { return m == Mode::kApart1 || m == Mode::kTogether1 ? 1 : 2; }
+// Rows of a workgroup against one source: kApart holds 16 in every wavefront,
+// kTogether1 and kTogether2 16 and 32 in each.
+enum class Mode { kApart, kTogether1, kTogether2 };
+constexpr bool together(Mode m) { return m != Mode::kApart; }
+constexpr int tiles_of(Mode m) { return m == Mode::kTogether2 ? 2 : 1; }
 constexpr uint32_t rows_of(Mode m) { return 16 * tiles_of(m) * (together(m) ? kWaves : 1); }
 
 // Wavefronts per SIMD that the registers are held to.
@@ -650,7 +694,7 @@ template <class T, int D, Mode M, Access A, Mode Kernel, class Limit>
 __device__ __forceinline__ void run_range(const Args& a, const Range& range, float (*shares)[16], Limit&& limit) {
   using Ops = Operands<T, D, A>;
   constexpr int QT = tiles_of(M);
-  Rows<Ops, QT> rows;
+  Rows<Ops, QT, together(M)> rows;
   const uint32_t first = together(M) ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 16 * QT : 0;
 #pragma unroll
   for (int t = 0; t < QT; ++t) rows.limit[t] = limit(min(first + 16 * t + threadIdx.x % 16, range.count - 1));
@@ -674,12 +718,10 @@ void k_ranges(const Args a) {
   uint32_t group, tile;
   if (blockIdx.x < a.prefix_blocks) {
     if (!block_task(blockIdx.x, a.kv_heads * a.prefix_splits, a.prefix_tiles, group, tile)) return;
-    range.kvh = group % a.kv_heads;
-    range.slot = group / a.kv_heads;
-    const uint32_t each = range_keys(a.prefix, a.prefix_splits);
-    range.begin = range.slot * each;
-    if (range.begin >= a.prefix) return;
-    range.end = range.least = min(range.begin + each, a.prefix);
+    range.kvh = group / a.prefix_splits;
+    range.slot = group % a.prefix_splits;
+    range.begin = range.slot * a.prefix_each;
+    range.end = range.least = min(range.begin + a.prefix_each, a.prefix);
     range.first = tile * rows_of(P);
     range.count = min(a.all_rows - range.first, rows_of(P));
     range.scores = nullptr;
@@ -690,8 +732,8 @@ void k_ranges(const Args a) {
     return;
   }
   if (!block_task(blockIdx.x - a.prefix_blocks, a.batch * a.kv_heads * a.own_splits, a.own_tiles, group, tile)) return;
-  range.kvh = group % a.kv_heads;
-  const uint32_t split = group / a.kv_heads % a.own_splits, b = group / a.kv_heads / a.own_splits;
+  const uint32_t split = group % a.own_splits, b = group / a.own_splits / a.kv_heads;
+  range.kvh = group / a.own_splits % a.kv_heads;
   range.slot = a.prefix_splits + split;
   const uint32_t n = length_of(a, b), each = range_keys(n, a.own_splits);
   range.begin = split * each;
@@ -713,18 +755,18 @@ void k_ranges(const Args a) {
 
 // The ranges that hold something of one row, in order.
 struct RowRanges {
-  uint32_t before, own, seen;
+  uint32_t own, seen;
   uint64_t step, base;
+  uint32_t before;
   __device__ __forceinline__ RowRanges(const Args& a, uint32_t kvh, uint32_t row, uint32_t n) {
     seen = visible(n, a.rows, row % a.seq_rows / a.group);
-    before = ranges_of(a.prefix, a.prefix_splits);
+    before = a.prefix_splits;
     own = seen ? (seen - 1) / range_keys(n, a.own_splits) + 1 : 0;  // ranges past the last key it sees hold nothing of it
     step = static_cast<uint64_t>(a.kv_heads) * a.all_rows;
     base = static_cast<uint64_t>(kvh) * a.all_rows + row;
-    skipped = a.prefix_splits - before;
   }
   __device__ __forceinline__ uint32_t count() const { return before + own; }
-  __device__ __forceinline__ uint64_t place(uint32_t r) const { return (r < before ? r : r + skipped) * step + base; }
+  __device__ __forceinline__ uint64_t place(uint32_t r) const { return r * step + base; }
   // Maximum (as subtracted) and sum over all ranges, by one wavefront.
   __device__ __forceinline__ float2 whole(const float2* part) const {
     const uint32_t lane = threadIdx.x % 64;
@@ -740,10 +782,9 @@ struct RowRanges {
     for (int off = 32; off; off /= 2) total = total + __shfl_xor(total, off);
     return make_float2(from, total);
   }
-
- private:
-  uint32_t skipped;
 };
+
+constexpr int kFewRanges = 8;
 
 // Joins the ranges of one row.  D / 4 lanes hold a row of a range, four
 // features each, so a wavefront reads 256 / D ranges at a time and a workgroup
@@ -755,16 +796,37 @@ __device__ __forceinline__ void join_row(const Args& a, uint32_t task, f32x4 (*r
   const uint32_t kvh = task % a.kv_heads, row = task / a.kv_heads;
   const RowRanges ranges(a, kvh, row, length_of(a, row / a.seq_rows));
   const uint32_t f = lane % kLanes * 4, first = wave * (64 / kLanes) + lane / kLanes;
-  const float2 whole = ranges.whole(a.part);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (f < a.pitch) {
-#pragma unroll 4
-    for (uint32_t r = first; r < ranges.count(); r += kAtOnce) {
-      const uint64_t at = ranges.place(r);
-      const f32x4 v = *reinterpret_cast<const f32x4*>(a.sums + at * a.pitch + f);
-      const float share = exp2_of(a.part[at].x - whole.x);
+  float2 whole;
+  auto add = [&](float share, uint64_t at) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(a.sums + at * a.pitch + f);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fma_rn(share, v[e], acc[e]);
+    for (int e = 0; e < 4; ++e) acc[e] = fma_rn(share, v[e], acc[e]);
+  };
+  if constexpr (W == 1) {  // at most kFewRanges: every lane has all maxima and sums
+    float2 part[kFewRanges];
+    float top = -INFINITY;
+    whole.y = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kFewRanges; ++r)
+      part[r] = static_cast<uint32_t>(r) < ranges.count() ? a.part[ranges.place(r)] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+    for (int r = 0; r < kFewRanges; ++r) top = fmaxf(top, part[r].x);
+    whole.x = reference_of(top);
+#pragma unroll
+    for (int r = 0; r < kFewRanges; ++r) {
+      const float share = exp2_of(part[r].x - whole.x);
+      whole.y = fma_rn(share, part[r].y, whole.y);
+      if (r % kAtOnce == static_cast<int>(first) && static_cast<uint32_t>(r) < ranges.count() && f < a.pitch) add(share, ranges.place(r));
+    }
+  } else {
+    whole = ranges.whole(a.part);
+    if (f < a.pitch) {
+#pragma unroll 4
+      for (uint32_t r = first; r < ranges.count(); r += kAtOnce) {
+        const uint64_t at = ranges.place(r);
+        add(exp2_of(a.part[at].x - whole.x), at);
+      }
     }
   }
 #pragma unroll
@@ -858,26 +920,83 @@ __global__ __launch_bounds__(kThreads) void k_weights(const Args a) {
 #pragma unroll
   for (int u = 0; u < NT; ++u) Ops::load_row(keys, min(16u * u + i16, n - key0 - 1) * stride + 16 * g, g, a.width, k[u]);
   float sum[NT][4] = {};
-  // The first row that sees key0: n - rows + i + 1 > key0.
-  const uint32_t from_row = static_cast<uint64_t>(key0) + a.rows > n ? key0 + a.rows - n : 0;
-  for (uint32_t r0 = from_row * a.group / 16 * 16 + 16 * wave; r0 < a.seq_rows; r0 += 16 * kWaves) {
-    const uint32_t in_seq = min(r0 + i16, a.seq_rows - 1), row = b * a.seq_rows + in_seq;
-    u32x4 q[1][Ops::kSteps];
-    Ops::load_row(reinterpret_cast<const char*>(static_cast<const T*>(a.query) + query_offset(a, row, kvh)), 16 * g, g, a.width, q[0]);
+  // Row j sees key k from j = (k + rows - n) group on: n - rows + j / group + 1 > k.
+  auto first_row = [&](uint32_t key) {
+    return static_cast<uint64_t>(key) + a.rows > n ? (key + a.rows - n) * a.group : 0u;
+  };
+  // The lane's row of a tile, 16 kWaves rows further every time, and its operands;
+  // past the last row they repeat it.
+  uint32_t r0 = first_row(key0) / 16 * 16 + 16 * wave;
+  uint32_t position = (r0 + i16) / a.group, in_group = (r0 + i16) % a.group;
+  const uint32_t position_step = 16 * kWaves / a.group, group_step = 16 * kWaves % a.group;
+  u32x4 q[1][Ops::kSteps];
+  float2 whole;
+  auto load_rows = [&] {
+    const bool real = position < a.rows;
+    const uint32_t at = real ? position : a.rows - 1, of = real ? in_group : a.group - 1;
+    const uint64_t row = static_cast<uint64_t>(b) * a.rows + at;
+    const T* src = static_cast<const T*>(a.query) + (row * a.q_heads + kvh * a.group + of) * a.width;
+    Ops::load_row(reinterpret_cast<const char*>(src), 16 * g, g, a.width, q[0]);
+    whole = a.whole[static_cast<uint64_t>(kvh) * a.all_rows + row * a.group + of];
+    position += position_step;
+    in_group += group_step;
+    if (in_group >= a.group) {
+      in_group -= a.group;
+      ++position;
+    }
+  };
+  f32x4 s[1][NT];
+  float from, inverse;
+  auto next_scores = [&] {
     take_sign<Ops>(scale, q[0]);
-    const float2 whole = a.whole[static_cast<uint64_t>(kvh) * a.all_rows + row];
-    f32x4 s[1][NT];
     Ops::scores(k, q, s);
-    const uint32_t seen = r0 + i16 < a.seq_rows ? visible(n, a.rows, in_seq / a.group) : 0;
-    const bool all = __all(seen >= key0 + kKeys);
+    from = -whole.x;
+    inverse = whole.y;
+    load_rows();
+  };
+  if (r0 < a.seq_rows) load_rows();
+  // Tiles in which some row does not see some key, or is past the last.
+  const uint32_t all_see = first_row(min(key0 + kKeys, n) - 1), step = 16 * kWaves;
+  uint32_t need[NT][4];
+#pragma unroll
+  for (int u = 0; u < NT; ++u)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t key = key0 + 16 * u + 4 * g + r;
+      need[u][r] = key < n ? first_row(key) : 0xffffffffu;
+    }
+  auto masked = [&] {
+    next_scores();
+    const uint32_t row = r0 + i16 < a.seq_rows ? r0 + i16 : 0;
 #pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float share = exp2_of(fma_rn(s[0][u][r], factor, -whole.x)) * whole.y;
-        if (all || key0 + 16 * u + 4 * g + r < seen) sum[u][r] = sum[u][r] + share;
-      }
+      for (int r = 0; r < 4; ++r)
+        if (r0 + i16 < a.seq_rows && row >= need[u][r])
+          sum[u][r] = fma_rn(exp2_of(fma_rn(s[0][u][r], factor, from)), inverse, sum[u][r]);
+  };
+  for (; r0 < a.seq_rows && (r0 < all_see || key0 + kKeys > n); r0 += step) masked();
+  // Whole tiles: the next one's products beside this one's exponentials.
+  if (r0 + 16 <= a.seq_rows) {
+    next_scores();
+    for (; r0 + step + 16 <= a.seq_rows; r0 += step) {
+      f32x4 now[NT];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) now[u] = s[0][u];
+      const float from_now = from, inverse_now = inverse;
+      next_scores();
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[u][r] = fma_rn(exp2_of(fma_rn(now[u][r], factor, from_now)), inverse_now, sum[u][r]);
+    }
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[u][r] = fma_rn(exp2_of(fma_rn(s[0][u][r], factor, from)), inverse, sum[u][r]);
+    r0 += step;
   }
+  if (r0 < a.seq_rows) masked();
 #pragma unroll
   for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -911,7 +1030,7 @@ uint64_t product(std::initializer_list<uint64_t> factors, uint64_t most, const c
 // Row tiles per workgroup, ranges and workspace of one call.
 struct Layout {
   Args args{};
-  Mode prefix_mode = Mode::kApart1, own_mode = Mode::kApart1;
+  Mode prefix_mode = Mode::kApart, own_mode = Mode::kApart;
   int features = 64;            // D
   bool weighted = false, stored = false;
   uint64_t part_bytes = 0, sums_bytes = 0, whole_bytes = 0, score_bytes = 0;
@@ -924,8 +1043,6 @@ struct Layout {
     args.prefix_tiles = static_cast<uint32_t>(ceil_div(args.all_rows, rows_of(prefix)));
     args.own_tiles = static_cast<uint32_t>(ceil_div(args.seq_rows, rows_of(own)));
   }
-  // 32 rows where D = 256 has registers for 16.
-  Mode apart(uint32_t rows) const { return rows <= 16 || features == 256 ? Mode::kApart1 : Mode::kApart2; }
   void count_blocks() {
     auto blocks = [&](std::initializer_list<uint64_t> groups, uint64_t tiles) {
       const uint64_t rounded = ceil_div(product(groups, kMostBlocks, kTooMany), 8) * 8;
@@ -963,19 +1080,22 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted) {
   // Few rows: every wavefront has them all.  More: 64, or where that still
   // fills the chip 128, a workgroup.
   auto mode_of = [&](uint32_t rows, uint64_t groups) {
-    if (rows <= 32) return l.apart(rows);
+    if (rows <= 32) return Mode::kApart;
     return l.features < 256 && ceil_div(rows, 128) * groups >= 512 ? Mode::kTogether2 : Mode::kTogether1;
   };
   const Mode own = mode_of(a.seq_rows, uint64_t{a.batch} * a.kv_heads * ceil_div(a.capacity, kRound));
   const Mode all = prefix ? mode_of(a.all_rows, a.kv_heads * ceil_div(prefix, kRound)) : own;
-  l.set_modes(all, a.seq_rows <= 16 ? Mode::kApart1 : all);
+  l.set_modes(all, a.seq_rows <= 32 ? Mode::kApart : all);
   // Ranges: as many workgroups as the chip holds at once, each with whole rounds of keys.
   const uint64_t held = 256 * (l.features == 256 ? 1 : l.features == 64 && tiles_of(all) == 1 ? 3 : 2);
   const double work = static_cast<double>(a.kv_heads) *
                       (static_cast<double>(a.prefix_tiles) * a.prefix +
                        static_cast<double>(a.batch) * a.own_tiles * a.capacity);
   const uint64_t each = std::max<uint64_t>(kRound, static_cast<uint64_t>(work / held));
-  a.prefix_splits = static_cast<uint32_t>(ceil_div(prefix, each));
+  if (prefix) {
+    a.prefix_each = range_keys(a.prefix, static_cast<uint32_t>(ceil_div(prefix, each)));
+    a.prefix_splits = static_cast<uint32_t>(ceil_div(prefix, a.prefix_each));
+  }
   a.own_splits = static_cast<uint32_t>(ceil_div(a.capacity, each));
   l.count_blocks();
   a.pitch = (a.width + 3) / 4 * 4;
@@ -998,29 +1118,25 @@ void launch(hipStream_t s, const Layout& l) {
   auto run = [&](auto prefix, auto own) {
     k_ranges<T, D, decltype(prefix)::value, decltype(own)::value, A><<<blocks, kThreads, 0, s>>>(a);
   };
+  using Apart = std::integral_constant<Mode, Mode::kApart>;
   auto run_own = [&](auto prefix) {
-    if (l.own_mode == Mode::kApart1)
-      run(prefix, std::integral_constant<Mode, Mode::kApart1>{});
+    if (l.own_mode == Mode::kApart)
+      run(prefix, Apart{});
     else
       run(prefix, prefix);
   };
-  if (l.prefix_mode == Mode::kApart1) {
-    run(std::integral_constant<Mode, Mode::kApart1>{}, std::integral_constant<Mode, Mode::kApart1>{});
-  } else if constexpr (A != Access::kElements) {
-    if constexpr (D != 256) {
-      if (l.prefix_mode == Mode::kApart2) run_own(std::integral_constant<Mode, Mode::kApart2>{});
-    }
-    if constexpr (std::is_same_v<T, uint16_t>) {
-      if (l.prefix_mode == Mode::kTogether1) run_own(std::integral_constant<Mode, Mode::kTogether1>{});
-      if constexpr (D != 256) {
-        if (l.prefix_mode == Mode::kTogether2) run_own(std::integral_constant<Mode, Mode::kTogether2>{});
-      }
-    }
+  if (l.prefix_mode == Mode::kApart) {
+    run(Apart{}, Apart{});
+  } else if constexpr (A != Access::kElements && std::is_same_v<T, uint16_t>) {
+    if (l.prefix_mode == Mode::kTogether1)
+      run_own(std::integral_constant<Mode, Mode::kTogether1>{});
+    else if constexpr (D != 256)
+      run_own(std::integral_constant<Mode, Mode::kTogether2>{});
   }
   // A workgroup per row where there are many ranges, else a wavefront.
   const uint32_t tasks = a.kv_heads * a.all_rows;
   const uint32_t fused = l.stored ? l.weight_blocks : 0;
-  if (a.prefix_splits + a.own_splits > 8) {
+  if (a.prefix_splits + a.own_splits > kFewRanges) {
     k_join<T, D, 4><<<tasks + fused, kThreads, 0, s>>>(a, tasks);
   } else {
     const uint32_t blocks_of_rows = static_cast<uint32_t>(ceil_div(tasks, kWaves));
@@ -1067,11 +1183,11 @@ void submit(dl_queue* queue, int dtype, const dl_batch_shape* shape, uint64_t pr
   const Access access = !pieces ? Access::kElements
                         : static_cast<int>(l.args.width) == l.features ? Access::kWhole
                                                                        : Access::kPieces;
-  // The shared tiles are 16-byte pieces of BF16.  FP32 rows and others run
-  // apart; the ranges, and with them the workspace, stay.
-  if (access == Access::kElements || (dtype == DL_F32 && together(l.prefix_mode))) {
-    const Mode mode = access == Access::kElements ? Mode::kApart1 : l.apart(32);
-    l.set_modes(mode, l.own_mode == Mode::kApart1 ? Mode::kApart1 : mode);
+  // The shared tiles are 16-byte pieces of BF16: FP32 rows, which the FP32
+  // matrix rate bounds, and others run apart; the ranges, and with them the
+  // workspace, stay.
+  if (access == Access::kElements || dtype == DL_F32) {
+    l.set_modes(Mode::kApart, Mode::kApart);
     l.count_blocks();
   }
   require(o.query && o.key && o.value && o.lengths && o.output && o.scale, "null operand");
