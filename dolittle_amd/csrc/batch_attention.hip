@@ -428,18 +428,12 @@ __device__ __forceinline__ void load_queries(const Args& a, const Range& range, 
   }
 }
 
-// Few rows: every wavefront holds all of them and takes every fourth step, its
-// keys and values straight from memory, a step ahead.
+// Few rows: every wavefront holds all of them and takes every fourth step,
+// its keys and values straight from memory, a step ahead.
 template <class Ops, int QT>
 struct Joined {
-  f32x4 o[2 * QT][Ops::C][64];
+  f32x4 o[kWaves / 2 * QT][Ops::C][64];
 };
-
-template <int Bytes>
-__device__ __forceinline__ uint8_t* joined_room() {
-  __shared__ __align__(16) uint8_t room[Bytes];
-  return room;
-}
 
 template <class T, int D, int QT, Access A>
 __device__ __forceinline__ void run_apart(const Args& a, const Range& range, Rows<Operands<T, D, A>, QT, false>& rows,
@@ -518,12 +512,12 @@ __device__ __forceinline__ void run_apart(const Args& a, const Range& range, Row
 #pragma unroll
   for (int t = 0; t < QT; ++t) rows.sum[t] = group_sum(rows.sum[t]);
 
-  // Join the wavefronts: 2 and 3 into 0 and 1, then 1 into 0; those without a
-  // step have nothing to give.  A giver's maxima and sums lie in its own shares.
+  // Join the wavefronts: the upper half into the lower, and so on; those without
+  // a step have nothing to give.  A giver's maxima and sums lie in its own shares.
   auto stats = [&](int of) { return reinterpret_cast<float2*>(shares + of * 32); };
   const uint32_t steps = end > range.begin ? (end - range.begin + KT - 1) / KT : 0;
 #pragma unroll
-  for (int half = 2; half; half /= 2) {
+  for (int half = kWaves / 2; half; half /= 2) {
     if (steps <= static_cast<uint32_t>(half)) continue;
     if (wave >= half && wave < 2 * half) {
 #pragma unroll
@@ -561,8 +555,7 @@ __device__ __forceinline__ void run_apart(const Args& a, const Range& range, Row
 template <int D>
 struct Stage {
   static constexpr int kKeys = D == 256 ? 32 : 64, kPieces = D / 8, kRowBytes = 2 * D;
-  static constexpr int kBytes = kKeys * kRowBytes;       // of keys, and of values
-  static constexpr int kLoads = kBytes / 1024 / kWaves;  // 1024-byte loads of a wavefront
+  static constexpr int kBytes = kKeys * kRowBytes;  // of keys, and of values
   static __device__ __forceinline__ uint32_t swizzle(uint32_t row) {
     return D == 64 ? 2 * (row / 2 % 4) + row / 8 % 2 : 2 * (row % 8) + row / 8 % 2;
   }
@@ -598,7 +591,7 @@ __device__ __forceinline__ void run_together(const Args& a, const Range& range, 
     const char* keys = range.keys + static_cast<uint64_t>(at) * stride;
     const char* values = range.values + static_cast<uint64_t>(at) * stride;
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) {
+    for (int i = 0; i < S::kBytes / 1024 / kWaves; ++i) {  // 1024 bytes of each at a time
       const uint32_t slot = (i * kWaves + wave) * 64 + lane, row = slot / S::kPieces;
       uint32_t piece = slot % S::kPieces ^ S::swizzle(row);
       if (A != Access::kWhole && piece * 8 >= width) piece = 0;  // not a piece of the row: cleared or not stored
@@ -690,6 +683,12 @@ constexpr int waves_per_simd() {
   return D == 256 ? 1 : D == 64 && tiles_of(M) == 1 ? 3 : 2;
 }
 
+template <class Room>
+__device__ __forceinline__ Room* joined_room() {
+  __shared__ __align__(16) Room room;
+  return &room;
+}
+
 template <class T, int D, Mode M, Access A, Mode Kernel, class Limit>
 __device__ __forceinline__ void run_range(const Args& a, const Range& range, float (*shares)[16], Limit&& limit) {
   using Ops = Operands<T, D, A>;
@@ -704,7 +703,7 @@ __device__ __forceinline__ void run_range(const Args& a, const Range& range, flo
     static_assert(sizeof(Joined<Ops, QT>) <= 2 * Stage<D>::kBytes, "joined outputs outgrow a stage");
     run_apart<T, D, QT, A>(a, range, rows, *reinterpret_cast<Joined<Ops, QT>*>(stage_room<D, 0>()), shares);
   } else {
-    run_apart<T, D, QT, A>(a, range, rows, *reinterpret_cast<Joined<Ops, QT>*>(joined_room<sizeof(Joined<Ops, tiles_of(Kernel)>)>()), shares);
+    run_apart<T, D, QT, A>(a, range, rows, *joined_room<Joined<Ops, QT>>(), shares);
   }
 }
 
@@ -1056,7 +1055,9 @@ struct Layout {
   }
 };
 
-Layout layout_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted) {
+// `pieces`: the rows are 16-byte pieces of BF16, which tiles can share.  Others
+// run apart: FP32 is bound by the FP32 matrix rate, not by its loads.
+Layout layout_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted, bool pieces) {
   check_shape(shape);
   require(prefix <= kMostKeys, "prefix too long", DL_LENGTH_ERROR);
   require(shape->width <= 256, "head width above 256", DL_LENGTH_ERROR);
@@ -1077,17 +1078,17 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted) {
   l.features = a.width <= 64 ? 64 : a.width <= 128 ? 128 : 256;
   l.weighted = weighted;
   l.stored = weighted && a.seq_rows <= 16;
-  // Few rows: every wavefront has them all.  More: 64, or where that still
-  // fills the chip 128, a workgroup.
-  auto mode_of = [&](uint32_t rows, uint64_t groups) {
-    if (rows <= 32) return Mode::kApart;
-    return l.features < 256 && ceil_div(rows, 128) * groups >= 512 ? Mode::kTogether2 : Mode::kTogether1;
+  // Few rows: every wavefront has them all.  More: 64 a workgroup, or 128 where
+  // those fill the chip (D = 256 has no registers for two tiles a wavefront).
+  auto mode_of = [&](uint32_t rows, uint64_t ranges) {
+    if (rows <= 32 || !pieces) return Mode::kApart;
+    return l.features < 256 && ceil_div(rows, 128) * ranges >= 512 ? Mode::kTogether2 : Mode::kTogether1;
   };
   const Mode own = mode_of(a.seq_rows, uint64_t{a.batch} * a.kv_heads * ceil_div(a.capacity, kRound));
   const Mode all = prefix ? mode_of(a.all_rows, a.kv_heads * ceil_div(prefix, kRound)) : own;
   l.set_modes(all, a.seq_rows <= 32 ? Mode::kApart : all);
   // Ranges: as many workgroups as the chip holds at once, each with whole rounds of keys.
-  const uint64_t held = 256 * (l.features == 256 ? 1 : l.features == 64 && tiles_of(all) == 1 ? 3 : 2);
+  const uint64_t held = 256 * (l.features == 256 ? 1 : l.features == 64 ? 3 : 2);
   const double work = static_cast<double>(a.kv_heads) *
                       (static_cast<double>(a.prefix_tiles) * a.prefix +
                        static_cast<double>(a.batch) * a.own_tiles * a.capacity);
@@ -1109,6 +1110,11 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted) {
   l.whole_bytes = room({a.kv_heads, a.all_rows, 8});
   l.score_bytes = l.stored ? room({a.kv_heads, a.all_rows, a.score_pitch, 4}) : 0;
   return l;
+}
+
+// Enough for either storage type and any alignment.
+uint64_t workspace_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted) {
+  return std::max(layout_of(shape, prefix, weighted, false).bytes(), layout_of(shape, prefix, weighted, true).bytes());
 }
 
 template <class T, int D, Access A>
@@ -1177,24 +1183,18 @@ struct Operation {
 
 void submit(dl_queue* queue, int dtype, const dl_batch_shape* shape, uint64_t prefix, const Operation& o, bool weighted) {
   require(dtype == DL_BF16 || dtype == DL_F32, "unsupported storage type");
-  Layout l = layout_of(shape, prefix, weighted);
+  check_shape(shape);
   const bool pieces =
       whole_pieces(shape, dtype == DL_BF16 ? 2 : 4, {o.query, o.prefix_key, o.prefix_value, o.key, o.value});
+  Layout l = layout_of(shape, prefix, weighted, pieces && dtype == DL_BF16);
   const Access access = !pieces ? Access::kElements
                         : static_cast<int>(l.args.width) == l.features ? Access::kWhole
                                                                        : Access::kPieces;
-  // The shared tiles are 16-byte pieces of BF16: FP32 rows, which the FP32
-  // matrix rate bounds, and others run apart; the ranges, and with them the
-  // workspace, stay.
-  if (access == Access::kElements || dtype == DL_F32) {
-    l.set_modes(Mode::kApart, Mode::kApart);
-    l.count_blocks();
-  }
   require(o.query && o.key && o.value && o.lengths && o.output && o.scale, "null operand");
   require(prefix == 0 || (o.prefix_key && o.prefix_value), "null prefix operand");
   require(!weighted || (o.weights && o.weights_out), "null weights");
   require(o.workspace != nullptr && reinterpret_cast<uintptr_t>(o.workspace) % 16 == 0, "workspace null or not 16-byte aligned");
-  require(o.workspace_bytes >= l.bytes(), "workspace too small", DL_LENGTH_ERROR);
+  require(o.workspace_bytes >= workspace_of(shape, prefix, weighted), "workspace too small", DL_LENGTH_ERROR);
   enter(queue);
   Args& a = l.args;
   a.query = o.query;
@@ -1230,14 +1230,14 @@ extern "C" {
 int dl_attention_shared_bytes(const dl_batch_shape* shape, uint64_t prefix, uint64_t* bytes) {
   return guard([&] {
     require(bytes != nullptr, "null output");
-    *bytes = dl::batch::layout_of(shape, prefix, false).bytes();
+    *bytes = dl::batch::workspace_of(shape, prefix, false);
   });
 }
 
 int dl_attention_weighted_bytes(const dl_batch_shape* shape, uint64_t prefix, uint64_t* bytes) {
   return guard([&] {
     require(bytes != nullptr, "null output");
-    *bytes = dl::batch::layout_of(shape, prefix, true).bytes();
+    *bytes = dl::batch::workspace_of(shape, prefix, true);
   });
 }
 
