@@ -833,6 +833,7 @@ __device__ __forceinline__ void join_row(const Args& a, uint32_t task, f32x4 (*r
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = acc[e] + __shfl_xor(acc[e], off);
   if constexpr (W > 1) {
+    __syncthreads();  // the row before is read
     room[wave][lane] = acc;
     __syncthreads();
     if (wave) return;
@@ -888,8 +889,9 @@ __global__ __launch_bounds__(kThreads) void k_join(const Args a, uint32_t join_b
   __shared__ f32x4 room[W == 1 ? 1 : W][64];
   __shared__ float2 stats[16];
   if (blockIdx.x < join_blocks) {
-    const uint32_t task = W == 1 ? blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : blockIdx.x;
-    if (task < a.kv_heads * a.all_rows) join_row<T, D, W>(a, task, room);
+    constexpr uint32_t kTasks = W == 1 ? kWaves : 1;  // of a block at once
+    uint32_t task = blockIdx.x * kTasks + (W == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);
+    for (; task < a.kv_heads * a.all_rows; task += join_blocks * kTasks) join_row<T, D, W>(a, task, room);
   } else {
     add_weights(a, blockIdx.x - join_blocks, stats);
   }
@@ -1015,7 +1017,8 @@ __global__ __launch_bounds__(kThreads) void k_weights(const Args a) {
 
 // ------------------------------------------------------------------- the host
 constexpr const char* kTooMany = "too many workgroups";
-constexpr uint64_t kMostBlocks = 1u << 30;
+// A launch's threads are counted in 32 bits; two kinds of blocks share one.
+constexpr uint64_t kMostBlocks = (1u << 23) - 8;
 
 uint64_t product(std::initializer_list<uint64_t> factors, uint64_t most, const char* what) {
   uint64_t p = 1;
@@ -1082,7 +1085,7 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted, bo
   // those fill the chip (D = 256 has no registers for two tiles a wavefront).
   auto mode_of = [&](uint32_t rows, uint64_t ranges) {
     if (rows <= 32 || !pieces) return Mode::kApart;
-    return l.features < 256 && ceil_div(rows, 128) * ranges >= 512 ? Mode::kTogether2 : Mode::kTogether1;
+    return l.features < 256 && rows > 64 && ceil_div(rows, 128) * ranges >= 512 ? Mode::kTogether2 : Mode::kTogether1;
   };
   const Mode own = mode_of(a.seq_rows, uint64_t{a.batch} * a.kv_heads * ceil_div(a.capacity, kRound));
   const Mode all = prefix ? mode_of(a.all_rows, a.kv_heads * ceil_div(prefix, kRound)) : own;
@@ -1142,10 +1145,12 @@ void launch(hipStream_t s, const Layout& l) {
   // A workgroup per row where there are many ranges, else a wavefront.
   const uint32_t tasks = a.kv_heads * a.all_rows;
   const uint32_t fused = l.stored ? l.weight_blocks : 0;
+  constexpr uint32_t kJoinBlocks = 1u << 22;
   if (a.prefix_splits + a.own_splits > kFewRanges) {
-    k_join<T, D, 4><<<tasks + fused, kThreads, 0, s>>>(a, tasks);
+    const uint32_t blocks_of_rows = std::min(tasks, kJoinBlocks);
+    k_join<T, D, 4><<<blocks_of_rows + fused, kThreads, 0, s>>>(a, blocks_of_rows);
   } else {
-    const uint32_t blocks_of_rows = static_cast<uint32_t>(ceil_div(tasks, kWaves));
+    const uint32_t blocks_of_rows = std::min(static_cast<uint32_t>(ceil_div(tasks, kWaves)), kJoinBlocks);
     k_join<T, D, 1><<<blocks_of_rows + fused, kThreads, 0, s>>>(a, blocks_of_rows);
   }
   if (l.weighted && !l.stored) k_weights<T, D, A><<<l.weight_blocks, kThreads, 0, s>>>(a);

@@ -494,7 +494,7 @@ int dl_cache_append(dl_queue* queue, int dtype, const dl_batch_shape* shape, con
     const AppendArgs a{query, key, value, query_out, keys, values, lengths, positions, lengths_out, positions_out, slots, weights,
                        shape->rows, shape->capacity, static_cast<uint32_t>(shape->query_heads),
                        static_cast<uint32_t>(shape->kv_heads), static_cast<uint32_t>(shape->width), theta};
-    const dim3 grid(static_cast<unsigned>(shape->rows), static_cast<unsigned>(shape->batch));
+    const dim3 grid(static_cast<unsigned>(std::min<uint64_t>(shape->rows, 1u << 20)), static_cast<unsigned>(shape->batch));
     if (dtype == DL_BF16)
       k_append<uint16_t><<<grid, kAppendThreads, 0, queue->stream>>>(a);
     else

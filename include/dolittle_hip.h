@@ -218,10 +218,12 @@ int dl_prefill_gate_up(dl_queue* queue, const void* input, const void* packed, v
  *   weights          FP32 [batch][kv_heads][capacity]: the attention that each
  *                    slot's row received
  * dtype is DL_BF16 or DL_F32.  Any element-aligned address and any width are
- * accepted; 16-byte aligned addresses and head rows run fastest.  What lies past a length is neither used nor
- * written.  No operation allocates, waits, or uses atomics on results: the
- * same call gives the same bits, and calls may be captured into graphs.  A
- * workspace belongs to one call at a time; its contents need not survive. */
+ * accepted; 16-byte aligned addresses and head rows run fastest.  Operands do
+ * not overlap except where an operation says that they may.  What lies past a
+ * length is neither used nor written.  No operation allocates, waits, or uses
+ * atomics on results: the same call gives the same bits, and calls may be
+ * captured into graphs.  A workspace (16-byte aligned) belongs to one call at a
+ * time; its contents need not survive. */
 typedef struct dl_batch_shape {
   uint64_t batch;       /* sequences */
   uint64_t rows;        /* new rows per sequence: 1 for a decode step */

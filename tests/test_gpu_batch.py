@@ -123,6 +123,19 @@ SHAPES = [
     (2, 3, 17, 37, (4, 2, 20), [37, 2]),
     (1, 18, 17, 37, (4, 2, 65), [37]),
     (1, 2, 33, 37, (3, 1, 255), [36]),
+    # Many rows, in BF16 64 or 128 a workgroup that shares its keys: prefix and
+    # own cache, both forms on one or the other, each width and piece count.
+    (1, 65, 0, 160, (4, 1, 128), [160]),
+    (70, 1, 300, 40, (4, 2, 128), [40 - b % 41 for b in range(70)]),
+    (40, 1, 129, 33, (6, 3, 96), [33 - b % 34 for b in range(40)]),
+    (9, 1, 700, 33, (8, 1, 256), [33, 0, 1, 2, 3, 32, 31, 30, 5]),
+    (5, 17, 100, 97, (3, 1, 248), [97, 17, 5, 96, 64]),
+    (1, 129, 1024, 320, (8, 8, 64), [320]),
+    (1, 140, 8200, 141, (8, 8, 64), [141]),
+    (3, 33, 8100, 40, (16, 8, 128), [40, 33, 1]),
+    (35, 1, 8192, 9, (16, 8, 88), [9 - b % 10 for b in range(35)]),
+    (2, 80, 0, 2100, (16, 8, 40), [2100, 81]),
+    (1, 150, 0, 4200, (16, 8, 128), [4133]),
 ]
 
 
@@ -317,6 +330,10 @@ EVICTIONS = [
     (1, 2, 8, 50, [50], (1 << 64) - 1, 1, (1 << 64) - 3),
     (1, 1, 8, 70000, [69999], 1500, 10, 40),
     (1, 1, 8, 70000, [70000], 69001, 10, 40),
+    (1, 2, 8, 36864, [36864], 20000, 0, 1),  # the longest cache whose keys are held on chip
+    (1, 2, 8, 36865, [36865], 20000, 0, 1),
+    (1, 2, 8, 1024, [1024], 512, 0, 1),
+    (1, 2, 8, 1025, [1025], 1024, 0, 1),
 ]
 
 
