@@ -136,6 +136,7 @@ SHAPES = [
     (35, 1, 8192, 9, (16, 8, 88), [9 - b % 10 for b in range(35)]),
     (2, 80, 0, 2100, (16, 8, 40), [2100, 81]),
     (1, 150, 0, 4200, (16, 8, 128), [4133]),
+    (17, 1, 8192, 3, (32, 8, 128), [3 - b % 4 for b in range(17)]),
 ]
 
 
@@ -481,3 +482,93 @@ def test_decode_with_bounded_caches(device, queue, oracle, dtype):
     assert cache.used == [int(x) for x in queue.read(cache.lengths, np.uint64, batch)]
     with pytest.raises(_lib.LengthError):
         cache.append(None, None, None, None, capacity)
+
+
+def test_steps_replayed_from_graphs(device, queue, oracle):
+    """Append, weighted attention and eviction recorded once into a sequence's
+    graphs and replayed nine times, twice, with eager work between: the bits of
+    the same steps submitted one by one."""
+    batch, prefix, capacity, budget, heads, steps = 3, 70, 9, 8, (8, 2, 64), 9
+    qh, kvh, w = heads
+    rng = np.random.default_rng(3)
+    make = lambda *s: stored(oracle, rng.standard_normal(s), "bf16")  # noqa: E731
+    pk, pv = (up(device, queue, make(prefix, kvh, w))[0] for _ in range(2))
+    q, k, v = (up(device, queue, make(batch, 1, h, w))[0] for h in (qh, kvh, kvh))
+    start = make(batch, capacity, kvh, w), make(batch, capacity, kvh, w)
+
+    class Side:
+        def __init__(self):
+            self.cache = BatchCache(device, queue, batch, capacity, qh, kvh, w, first_position=prefix)
+            for buf, x in zip((self.cache.keys, self.cache.values), start):
+                queue.write(buf, x)
+            for buf in (self.cache.weights, self.cache.slots):
+                queue.write(buf, np.zeros(batch * kvh * capacity, np.float32))
+            self.turned, self.out = (device.allocate(batch * qh * w * 2) for _ in range(2))
+            shape = self.cache.shape()
+            rooms = [workspace_bytes("dl_attention_weighted", shape, prefix), workspace_bytes("dl_cache_evict", shape, budget)]
+            self.work = [device.upload_array(queue, np.full(n, 0xFF, np.uint8)) for n in rooms]
+
+        def step(self):
+            c, shape = self.cache, self.cache.shape()
+            _lib.call("dl_cache_append", queue.handle, 1, C.byref(shape), q.ptr(), k.ptr(), v.ptr(), self.turned.ptr(),
+                      c.keys.ptr(), c.values.ptr(), c.lengths.ptr(), c.lengths.ptr(), c.positions.ptr(), c.positions.ptr(),
+                      c.slots.ptr(), c.weights.ptr(), 1e6)
+            _lib.call("dl_attention_weighted", queue.handle, 1, C.byref(shape), self.turned.ptr(), pk.ptr(), pv.ptr(), prefix,
+                      c.keys.ptr(), c.values.ptr(), c.lengths.ptr(), c.weights.ptr(), c.weights.ptr(), self.out.ptr(),
+                      c._scale.ptr(), self.work[0].ptr(), self.work[0].nbytes)
+            _lib.call("dl_cache_evict", queue.handle, 1, C.byref(shape), c.keys.ptr(), c.values.ptr(), c.lengths.ptr(),
+                      c.lengths.ptr(), c.slots.ptr(), c.slots.ptr(), c.weights.ptr(), c.weights.ptr(), budget, 1, 2,
+                      self.work[1].ptr(), self.work[1].nbytes)
+
+        def state(self):
+            c = self.cache
+            return [queue.read(b, np.uint8, b.nbytes) for b in (c.keys, c.values, c.weights, c.slots, c.lengths, c.positions,
+                                                                self.out)]
+
+    eager, replayed = Side(), Side()
+    ids = device.upload_array(queue, np.arange(steps, dtype=np.uint32))
+    token = device.allocate(4)
+    for _ in range(2):
+        handle = C.c_void_p()
+        _lib.call("dl_sequence_create", queue.handle, steps, 0, 1, 1, C.byref(handle))
+        try:
+            _lib.call("dl_sequence_begin", handle, None, None, token.ptr(), 4, ids.ptr(), steps * 4, None, None, None, None)
+            for stage in range(4):
+                _lib.call("dl_sequence_begin_stage", handle, stage)
+                if stage == 0:
+                    replayed.step()
+                if stage == 3:
+                    _lib.call("dl_sequence_begin_selection", handle)
+                _lib.call("dl_sequence_end_stage", handle)
+            _lib.call("dl_sequence_complete", handle)
+            _lib.call("dl_sequence_start", handle)
+            _lib.call("dl_sequence_drain", handle)
+        finally:
+            _lib.call("dl_sequence_destroy", handle)
+        for _ in range(steps):
+            eager.step()
+        queue.drain()
+        for got, want in zip(replayed.state(), eager.state()):
+            assert np.array_equal(got, want)
+    assert list(queue.read(eager.cache.positions, np.uint64, batch)) == [prefix + 2 * steps] * batch
+
+
+def test_cache_object_refusals(device, queue):
+    from dolittle_amd import InvalidArgument, LengthError
+    for bad in (dict(batch=0), dict(capacity=0), dict(width=0), dict(dtype="f16"), dict(first_position=-1)):
+        with pytest.raises(InvalidArgument):
+            BatchCache(device, queue, **{**dict(batch=1, capacity=4, query_heads=2, kv_heads=1, width=8), **bad})
+    cache = BatchCache(device, queue, 1, 4, 2, 1, 8)
+    x = device.allocate(256)
+    with pytest.raises(LengthError):
+        cache.append(x, x, x, x, 5)
+    with pytest.raises(InvalidArgument):
+        cache.append(x, x, x, x, 0)
+    with pytest.raises(InvalidArgument):
+        cache.append(None, x, x, x)
+    assert cache.used == [0]
+    for budget, sinks, recent in ((0, 0, 0), (3, 2, 2), (3, -1, 0)):
+        with pytest.raises(InvalidArgument):
+            cache.evict(budget, sinks, recent)
+    with pytest.raises(InvalidArgument):
+        cache.attend(None, x)
