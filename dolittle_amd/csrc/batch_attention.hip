@@ -10,19 +10,32 @@
 //
 // Split.  All rows of a KV head (every sequence's, every new row's, the heads
 // of the group) are one matrix against the prefix, so the prefix is read once
-// per 16 QT rows and not once per sequence.  A workgroup takes 16 QT rows and a
-// range of keys of one source (the prefix, or one sequence's cache); its four
-// wavefronts take every fourth step of keys and keep a running maximum, sum
-// and output of their own, joined at the end.  k_join joins the ranges.
+// for a workgroup's rows and not once per sequence.  A workgroup takes some
+// rows and a range of keys of one source (the prefix, or one sequence's cache)
+// and leaves their maximum, sum and unnormalised output; k_join joins the
+// ranges and adds up the weights of a decode step from the scores that k_ranges
+// stored; k_weights computes those of more rows again.
 //
-// Matrix operands, without a pass through LDS.  Scores are computed as K Q^T:
-// the first operand is K with a lane per key, so K is loaded straight from its
-// rows, and the result leaves a lane with scores of one row and the keys that
-// the second product's P^T operand wants from it.  That product is V^T P^T:
-// a lane loads C = D / 16 neighbouring features of the keys it contracts, and
-// since any 16 features may form a matrix tile, tile j takes feature j of each
-// lane's C: the transposition is a byte permute of two registers (BF16) or
-// nothing (FP32).
+// Up to 32 rows, FP32 rows and rows that are not 16-byte pieces run apart: 16
+// in every wavefront, the wavefronts taking every fourth step of 32 keys (FP32
+// 16) straight from memory into matrix operands.  Scores are K Q^T, so that the
+// first operand has a lane per key, and leave a lane with the keys that the
+// P^T operand of V^T P^T wants from it; a lane loads C = D / 16 neighbouring
+// features of each of its keys, and since any 16 features may form a matrix
+// tile, tile j takes feature j of every lane's C: the transposition is a byte
+// permute (BF16) or nothing (FP32).  Bound by the key and value stream: 8
+// sequences of up to 4607 keys, 101 MB in 26 us, of which 4 until the first
+// step has landed (6.15 TB/s is this card's rate for a large read).  FP32 is
+// bound by its matrix rate: 48 rows a KV head over 1001 keys 19 us, 6 at 154
+// TFLOP/s; what is more is the first loads and two workgroups to a SIMD.
+//
+// More BF16 rows run together: 16 or 32 in each wavefront, keys and values
+// through LDS for all four (64 sequences over 32768 keys 84 us, 114 with every
+// wavefront loading its own).  Bound by the issue of vector instructions beside
+// the matrix products, two wavefronts to a SIMD: a step of 32 rows and 32 keys
+// takes about 1050 cycles, 512 of them products (512 rows of 4 heads over 4096
+// keys 52 us, 630 TFLOP/s).  Which form is taken goes by rows and storage
+// alone; 128 rows a workgroup instead of 64 where those still fill the chip.
 //
 // BF16 storage rounds P to BF16 (8 bits, relative 2^-9) for the product with V;
 // scores, exponentials, sums, maxima and outputs are FP32 throughout, and so
@@ -785,7 +798,9 @@ struct RowRanges {
 
 constexpr int kFewRanges = 8;
 
-// Joins the ranges of one row.  D / 4 lanes hold a row of a range, four
+// Joins the ranges of one row (4 us where there are few rows, most of it launch
+// and the wait for the first loads; 12 us for 16,384 rows of four ranges, 34
+// MB).  D / 4 lanes hold a row of a range, four
 // features each, so a wavefront reads 256 / D ranges at a time and a workgroup
 // of W = 4 four times as many: the loads of a row are a few deep.
 template <class T, int D, int W>
@@ -844,9 +859,18 @@ __device__ __forceinline__ void join_row(const Args& a, uint32_t task, f32x4 (*r
   if (lane >= kLanes) return;
   T* out = static_cast<T*>(a.out) + query_offset(a, row, kvh);
   const bool none = a.prefix + ranges.seen == 0;
+  struct alignas(4 * sizeof(T)) Four {
+    T v[4];
+  } four;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (f + e < a.width) store_elem(out, f + e, none ? 0.0f : acc[e] / whole.y);
+  for (int e = 0; e < 4; ++e) store_elem(four.v, e, none ? 0.0f : acc[e] / whole.y);
+  if (a.width % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % sizeof four == 0) {
+    if (f < a.width) *reinterpret_cast<Four*>(out + f) = four;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (f + e < a.width) out[f + e] = four.v[e];
+  }
 }
 
 // Weights of up to 16 rows from their stored scores: a thread sums four
@@ -898,7 +922,8 @@ __global__ __launch_bounds__(kThreads) void k_join(const Args a, uint32_t join_b
 }
 
 // Weights of more rows: the scores again, a workgroup per 16 NT keys, held in
-// registers.  The wavefronts walk every fourth tile of the rows that see them;
+// registers (2048 rows over 4096 keys, 8 KV heads: 42 us, 8 of products; the
+// query loads cost 15, the exponentials 2).  The wavefronts walk every fourth tile of the rows that see them;
 // a lane sums its keys over its rows, then the lanes and the wavefronts add up
 // in a fixed order.  Every key has one owner: no atomics.
 template <class T, int D, Access A>

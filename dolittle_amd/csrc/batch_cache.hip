@@ -7,6 +7,7 @@
 // its position and its accumulated weight in [batch][kv_heads][capacity].
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "batch.h"
 #include "dl_device.h"
@@ -42,11 +43,19 @@ __device__ __forceinline__ void advance(const AppendArgs& a, uint64_t b) {
 // FP32 and a rotated value is rounded once, where the catalog's rotary rounds
 // cosine, sine and each product to the storage type (0.26% against 0.17% off in
 // BF16; the same bits in FP32).  Bound: the chain of 64-bit operations of one angle.
-template <class T>
-__global__ __launch_bounds__(kAppendThreads) void k_append(const AppendArgs a) {
-  __shared__ float cosine[kAppendPairs], sine[kAppendPairs];
+template <class T, int N>
+struct alignas(N * sizeof(T)) Pack {
+  T v[N];
+};
+
+// N features of a head at a time: 4 where halves of a head are whole packs of
+// 4 and the operands lie on their boundaries, else 1.
+template <class T, int N>
+__global__ __launch_bounds__(kAppendThreads) void k_append(const AppendArgs a, bool advance_here) {
+  using Features = Pack<T, N>;
+  __shared__ __align__(16) float cosine[kAppendPairs], sine[kAppendPairs];
   const uint64_t b = blockIdx.y;
-  const uint32_t half = a.width / 2;
+  const uint32_t half = a.width / 2, packs = half / N;
   const uint64_t n = a.lengths[b], first = a.positions[b];
   for (uint64_t i = blockIdx.x; i < a.rows; i += gridDim.x) {
     const uint64_t position = first + i, slot = n + i, row = b * a.rows + i;
@@ -61,24 +70,30 @@ __global__ __launch_bounds__(kAppendThreads) void k_append(const AppendArgs a) {
       sine[f] = static_cast<float>(s);
     }
     __syncthreads();
-    auto turn = [&](const T* x, T* y, uint32_t f) {
-      const float lo = load_elem(x, f), hi = load_elem(x, f + half), c = cosine[f], s = sine[f];
-      store_elem(y, f, lo * c - hi * s);
-      store_elem(y, f + half, hi * c + lo * s);
+    auto turn = [&](const T* x, T* y, uint32_t heads) {
+      for (uint32_t p = threadIdx.x; p < heads * packs; p += kAppendThreads) {
+        const uint32_t at = p / packs * a.width, f = p % packs * N;
+        const Features lo = *reinterpret_cast<const Features*>(x + at + f), hi = *reinterpret_cast<const Features*>(x + at + half + f);
+        Features lo_out, hi_out;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float u = load_elem(lo.v, e), v = load_elem(hi.v, e), c = cosine[f + e], s = sine[f + e];
+          store_elem(lo_out.v, e, u * c - v * s);
+          store_elem(hi_out.v, e, v * c + u * s);
+        }
+        *reinterpret_cast<Features*>(y + at + f) = lo_out;
+        *reinterpret_cast<Features*>(y + at + half + f) = hi_out;
+      }
     };
-    const T* query = static_cast<const T*>(a.query) + row * a.q_heads * a.width;
-    T* query_out = static_cast<T*>(a.query_out) + row * a.q_heads * a.width;
-    for (uint32_t p = threadIdx.x; p < a.q_heads * half; p += kAppendThreads)
-      turn(query + p / half * a.width, query_out + p / half * a.width, p % half);
+    const uint64_t query_at = row * a.q_heads * a.width;
+    turn(static_cast<const T*>(a.query) + query_at, static_cast<T*>(a.query_out) + query_at, a.q_heads);
     if (fits) {
-      const uint64_t key_width = static_cast<uint64_t>(a.kv_heads) * a.width;
-      const T* key = static_cast<const T*>(a.key) + row * key_width;
-      const T* value = static_cast<const T*>(a.value) + row * key_width;
-      T* to_key = static_cast<T*>(a.keys) + (b * a.capacity + slot) * key_width;
-      T* to_value = static_cast<T*>(a.values) + (b * a.capacity + slot) * key_width;
-      for (uint32_t p = threadIdx.x; p < a.kv_heads * half; p += kAppendThreads)
-        turn(key + p / half * a.width, to_key + p / half * a.width, p % half);
-      for (uint32_t f = threadIdx.x; f < key_width; f += kAppendThreads) to_value[f] = value[f];
+      const uint32_t key_width = a.kv_heads * a.width;
+      const uint64_t from = row * key_width, to = (b * a.capacity + slot) * key_width;
+      turn(static_cast<const T*>(a.key) + from, static_cast<T*>(a.keys) + to, a.kv_heads);
+      const Features* value = reinterpret_cast<const Features*>(static_cast<const T*>(a.value) + from);
+      Features* to_value = reinterpret_cast<Features*>(static_cast<T*>(a.values) + to);
+      for (uint32_t f = threadIdx.x; f < key_width / N; f += kAppendThreads) to_value[f] = value[f];
       for (uint32_t h = threadIdx.x; h < a.kv_heads; h += kAppendThreads) {
         const uint64_t at = (b * a.kv_heads + h) * a.capacity + slot;
         a.slots[at] = static_cast<uint32_t>(position);
@@ -87,9 +102,7 @@ __global__ __launch_bounds__(kAppendThreads) void k_append(const AppendArgs a) {
     }
     __syncthreads();
   }
-  // A sequence of one workgroup advances here: it has read its length, which
-  // lengths_out may be.
-  if (gridDim.x == 1 && threadIdx.x == 0) advance(a, b);
+  if (advance_here && blockIdx.x == 0 && threadIdx.x == 0) advance(a, b);
 }
 
 __global__ __launch_bounds__(64) void k_advance(const AppendArgs a, uint64_t batch) {
@@ -139,9 +152,11 @@ __device__ __forceinline__ uint64_t lane_of(uint64_t v, uint32_t lane) {
 // and the later ones count few keys.  Then a wavefront takes consecutive groups
 // of 64 slots, so that its ranks are running sums of population counts, from
 // one sum over the wavefronts.  Bound: the chain of barriers and of LDS and
-// instruction latency.  Keys in registers by thread, 40 unrolled, read the
-// operands at a stride and fetch five times the code: 81 us for 64 heads of
-// 32768 rows, 16 for 2049.
+// instruction latency, one compute unit to a head: of 36 us for 32768 rows 12
+// are the two reads, 15 the histograms, 8 masks and lists (of 8 us for 2049
+// rows 2.7, 5.6 and 3).  Keys in registers by thread, 40 unrolled, read the
+// operands at a stride and fetched five times the code: 81 us against 44 for
+// the launch.
 constexpr uint32_t kHeldKeys = 36 * 1024;
 
 template <int Threads, bool Held>
@@ -495,11 +510,23 @@ int dl_cache_append(dl_queue* queue, int dtype, const dl_batch_shape* shape, con
                        shape->rows, shape->capacity, static_cast<uint32_t>(shape->query_heads),
                        static_cast<uint32_t>(shape->kv_heads), static_cast<uint32_t>(shape->width), theta};
     const dim3 grid(static_cast<unsigned>(std::min<uint64_t>(shape->rows, 1u << 20)), static_cast<unsigned>(shape->batch));
+    // A sequence's only workgroup has read its length before it writes the new
+    // one, which may be the same word; of several any may still have to.
+    const bool apart = lengths != lengths_out && positions != positions_out && lengths != positions_out && positions != lengths_out;
+    const bool advance_here = grid.x == 1 || apart;
+    uintptr_t low = shape->width / 2 % 4;
+    for (const void* p : {query, key, value, static_cast<const void*>(query_out), static_cast<const void*>(keys), static_cast<const void*>(values)})
+      low |= reinterpret_cast<uintptr_t>(p) % (dtype == DL_BF16 ? 8 : 16);
+    auto run = [&](auto type, auto count) {
+      k_append<decltype(type), decltype(count)::value><<<grid, kAppendThreads, 0, queue->stream>>>(a, advance_here);
+    };
+    using Four = std::integral_constant<int, 4>;
+    using One = std::integral_constant<int, 1>;
     if (dtype == DL_BF16)
-      k_append<uint16_t><<<grid, kAppendThreads, 0, queue->stream>>>(a);
+      low ? run(uint16_t{}, One{}) : run(uint16_t{}, Four{});
     else
-      k_append<float><<<grid, kAppendThreads, 0, queue->stream>>>(a);
-    if (grid.x > 1)
+      low ? run(float{}, One{}) : run(float{}, Four{});
+    if (!advance_here)
       k_advance<<<static_cast<unsigned>(dl::ceil_div(shape->batch, 64)), 64, 0, queue->stream>>>(a, shape->batch);
     dl::check_launch(queue, "cache_append");
   });
