@@ -34,8 +34,10 @@ class BatchCache:
 
     The host keeps each sequence's length (append and evict change them by rules
     that need no device value), so a row that does not fit is refused here.
-    Every method only enqueues; `query` and the rows are device addresses or
-    buffers, [batch][rows][heads][width].
+    Every method only enqueues, except that a first attend or evict that needs
+    more workspace allocates it: run a step once before it is recorded into a
+    graph, and add a replayed step's rows to `used`.  `query` and the rows are
+    device addresses or buffers, [batch][rows][heads][width].
     """
 
     def __init__(self, device: Device, queue: Queue, batch: int, capacity: int, query_heads: int, kv_heads: int,
@@ -57,7 +59,7 @@ class BatchCache:
         _lib.call("dl_attention_scale", queue.handle, self._scale.ptr(), width)
         self.used = [0] * batch
         self._prefix = (None, None, 0)
-        self._work: DeviceBuffer | None = None
+        self._work: list[DeviceBuffer] = []
 
     def shape(self, rows: int = 1) -> BatchShape:
         qh, kvh, w = self._dims
@@ -100,13 +102,11 @@ class BatchCache:
         self.used = [min(n, budget) for n in self.used]
 
     def _workspace(self, need: int) -> tuple[C.c_void_p, int]:
-        """One workspace for the queue's operations, which run in order; grown after the queue has drained."""
-        if self._work is None or self._work.nbytes < need:
-            if self._work is not None:
-                self.queue.drain()
-                self._work.free()
-            self._work = self.device.allocate(need)
-        return self._work.ptr(), self._work.nbytes
+        """One workspace for the queue's operations, which run in order.  Smaller ones that it outgrew are kept,
+        for submitted and recorded work still uses them; each is at least twice the last."""
+        if not self._work or self._work[-1].nbytes < need:
+            self._work.append(self.device.allocate(max(need, 2 * self._work[-1].nbytes if self._work else 0)))
+        return self._work[-1].ptr(), self._work[-1].nbytes
 
 
 def _at(operand):

@@ -27,7 +27,7 @@
 // sequences of up to 4607 keys, 101 MB in 26 us, of which 4 until the first
 // step has landed (6.15 TB/s is this card's rate for a large read).  FP32 is
 // bound by its matrix rate: 48 rows a KV head over 1001 keys 19 us, 6 at 154
-// TFLOP/s; what is more is the first loads and two workgroups to a SIMD.
+// TFLOP/s; what is more is the first loads and two workgroups to a compute unit.
 //
 // More BF16 rows run together: 16 or 32 in each wavefront, keys and values
 // through LDS for all four (64 sequences over 32768 keys 84 us, 114 with every

@@ -32,9 +32,9 @@ struct AppendArgs {
 constexpr int kAppendThreads = 256, kAppendPairs = 2048;
 
 __device__ __forceinline__ void advance(const AppendArgs& a, uint64_t b) {
-  const uint64_t n = a.lengths[b] < a.capacity ? a.lengths[b] : a.capacity, grown = n + a.rows;
+  const uint64_t n = a.lengths[b] < a.capacity ? a.lengths[b] : a.capacity, grown = n + a.rows, first = a.positions[b];
   a.lengths_out[b] = grown < a.capacity ? grown : a.capacity;
-  a.positions_out[b] = a.positions[b] + a.rows;
+  a.positions_out[b] = first + a.rows;
 }
 
 // One workgroup per new row.  The rotation's angles depend on the position and
@@ -477,6 +477,7 @@ struct EvictLayout {
 EvictLayout evict_layout(const dl_batch_shape* shape, uint64_t budget) {
   check_shape(shape);
   require(budget > 0, "empty budget");
+  require(shape->batch * shape->kv_heads <= 65535, "too many sequences", DL_LENGTH_ERROR);
   const bool cuts = budget < shape->capacity;
   return {shape->batch * shape->kv_heads, cuts ? std::min(budget, shape->capacity - budget) : 0, cuts ? dl::ceil_div(budget, 64) : 0};
 }
@@ -549,7 +550,6 @@ int dl_cache_evict(dl_queue* queue, int dtype, const dl_batch_shape* shape, void
     const EvictLayout l = evict_layout(shape, budget);
     require(keys && values && lengths && lengths_out && slots && slots_out && weights && weights_out, "null operand");
     require(sinks <= budget && recent <= budget - sinks, "sinks and recent rows exceed the budget");
-    require(l.heads <= 65535, "too many sequences", DL_LENGTH_ERROR);
     require(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 8 == 0, "workspace null or not 8-byte aligned");
     require(workspace_bytes >= l.bytes(), "workspace too small", DL_LENGTH_ERROR);
     dl::enter(queue);

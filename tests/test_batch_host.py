@@ -157,3 +157,44 @@ def test_evict_workspace_follows_the_most_rows_that_can_move():
     for budget, most in ((1, 1), (8, 8), (16, 16), (31, 1), (32, 0), (1000, 0)):
         assert workspace_bytes("dl_cache_evict", shape(), budget) >= 4 * 4 * 2 * most
     assert workspace_bytes("dl_cache_evict", shape(capacity=1 << 20), 1 << 20) < 256  # nothing can move
+
+
+def test_evict_workspace_refuses_what_the_eviction_refuses():
+    with pytest.raises(LengthError, match="sequences"):
+        workspace_bytes("dl_cache_evict", shape(batch=40000), 8)
+    assert workspace_bytes("dl_cache_evict", shape(batch=65535, kv_heads=1), 8) > 0
+
+
+def test_an_outgrown_workspace_stays_allocated():
+    """Work recorded into a graph with the first workspace still writes to it
+    after a later call needed more."""
+    from dolittle_amd.batch import BatchCache
+
+    class Buffer:
+        freed = False
+
+        def __init__(self, nbytes):
+            self.nbytes = nbytes
+
+        def ptr(self):
+            return id(self)
+
+        def free(self):
+            self.freed = True
+
+    class Owner:
+        made = []
+
+        def allocate(self, nbytes):
+            self.made.append(Buffer(nbytes))
+            return self.made[-1]
+
+        def drain(self):
+            pass
+
+    cache = BatchCache.__new__(BatchCache)
+    cache.device = cache.queue = owner = Owner()
+    cache._work = []
+    kept = [cache._workspace(need) for need in (100, 50, 101, 200, 1000)]
+    assert [room for _, room in kept] == [100, 100, 200, 200, 1000]
+    assert len(owner.made) == 3 and not any(b.freed for b in owner.made)

@@ -374,6 +374,39 @@ def test_evict_orders(device, queue, oracle, kind):
             assert np.array_equal(g.view(np.uint8), e.view(np.uint8)), (name, budget)
 
 
+def test_evict_signalling_nan_weights(device, queue, oracle):
+    """Every NaN orders as -infinity, whatever its bits."""
+    k, v, w, s = evict_inputs(oracle, "bf16", 2, 1, 16, 500, 6)
+    bits = np.array([0x7f800001, 0x7fbfffff, 0x7fffffff, 0xff800001, 0xffffffff, 0xffc00000], np.uint32)
+    rng = np.random.default_rng(10)
+    at = rng.random(w.shape) < 0.5
+    w.view(np.uint32)[at] = rng.choice(bits, at.sum())
+    lengths = np.array([500, 333], np.uint64)
+    for budget in (100, 250, 480):
+        got = run_evict(device, queue, "bf16", k, v, w, s, lengths, budget, 2, 9, False)
+        want = want_evict(k, v, w, s, lengths, budget, 2, 9, False)
+        for name, g, e in zip(("keys", "values", "weights", "slots", "lengths"), got, want):
+            assert np.array_equal(g.view(np.uint8), e.view(np.uint8)), (name, budget)
+
+
+@pytest.mark.parametrize("same", ["weights", "slots", "lengths"])
+def test_evict_one_operand_in_place(device, queue, oracle, same):
+    k, v, w, s = evict_inputs(oracle, "f32", 2, 2, 12, 90, 7)
+    lengths, budget = np.array([90, 61], np.uint64), 50
+    shape = BatchShape(2, 1, 2, 2, 12, 90)
+    b = {n: up(device, queue, x) for n, x in dict(k=k, v=v, lengths=lengths, slots=s, weights=w).items()}
+    for n, x in dict(lengths=lengths, slots=s, weights=w).items():
+        b[n + "2"] = b[n] if n == same else up(device, queue, x)
+    room = workspace_bytes("dl_cache_evict", shape, budget)
+    work = device.allocate(room)
+    order = ("k", "v", "lengths", "lengths2", "slots", "slots2", "weights", "weights2")
+    _lib.call("dl_cache_evict", queue.handle, 2, C.byref(shape), *[b[n][1] for n in order], budget, 1, 5, work.ptr(), room)
+    queue.drain()
+    want = want_evict(k, v, w, s, lengths, budget, 1, 5, True)
+    for n, e in zip(("k", "v", "weights2", "slots2", "lengths2"), want):
+        assert np.array_equal(queue.read(b[n][0], e.dtype, e.size).reshape(e.shape).view(np.uint8), e.view(np.uint8)), n
+
+
 # --------------------------------------------------------------------- append
 APPENDS = [
     # batch, rows, capacity, (query heads, KV heads, width), lengths, positions
