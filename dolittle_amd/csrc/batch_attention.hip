@@ -782,11 +782,12 @@ struct RowRanges {
   // Maximum (as subtracted) and sum over all ranges, by one wavefront.
   __device__ __forceinline__ float2 whole(const float2* part) const {
     const uint32_t lane = threadIdx.x % 64;
-    float top = -INFINITY;
-    for (uint32_t r = lane; r < count(); r += 64) top = fmaxf(top, part[place(r)].x);
+    const float2 own_part = lane < count() ? part[place(lane)] : make_float2(-INFINITY, 0.0f);
+    float top = own_part.x;
+    for (uint32_t r = lane + 64; r < count(); r += 64) top = fmaxf(top, part[place(r)].x);
     const float from = reference_of(wave_max(top));
-    float total = 0.0f;
-    for (uint32_t r = lane; r < count(); r += 64) {
+    float total = exp2_of(own_part.x - from) * own_part.y;
+    for (uint32_t r = lane + 64; r < count(); r += 64) {
       const float2 p = part[place(r)];
       total = fma_rn(exp2_of(p.x - from), p.y, total);
     }
@@ -808,40 +809,62 @@ __device__ __forceinline__ void join_row(const Args& a, uint32_t task, f32x4 (*r
   constexpr int kLanes = D / 4, kAtOnce = W * 64 / kLanes;
   const int lane = threadIdx.x % 64, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t kvh = task % a.kv_heads, row = task / a.kv_heads;
-  const RowRanges ranges(a, kvh, row, length_of(a, row / a.seq_rows));
   const uint32_t f = lane % kLanes * 4, first = wave * (64 / kLanes) + lane / kLanes;
+  // What the first ranges left is read before the length says which of them hold
+  // something: one wait and not three.
+  const uint32_t all = a.prefix_splits + a.own_splits;
+  const uint64_t step = static_cast<uint64_t>(a.kv_heads) * a.all_rows, base = static_cast<uint64_t>(kvh) * a.all_rows + row;
+  const float* sums = a.sums + (f < a.pitch ? f : 0);
+  constexpr int kAhead = W == 1 ? (kFewRanges + kAtOnce - 1) / kAtOnce : 4;
+  f32x4 ahead[kAhead];
+#pragma unroll
+  for (int m = 0; m < kAhead; ++m) {
+    ahead[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (static_cast<uint32_t>(m) * kAtOnce < all)
+      ahead[m] = *reinterpret_cast<const f32x4*>(sums + (min(m * kAtOnce + first, all - 1) * step + base) * a.pitch);
+  }
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  float2 whole;
-  auto add = [&](float share, uint64_t at) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(a.sums + at * a.pitch + f);
+  auto add = [&](float share, const f32x4& v) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = fma_rn(share, v[e], acc[e]);
   };
+  float2 whole;
+  uint32_t seen;
   if constexpr (W == 1) {  // at most kFewRanges: every lane has all maxima and sums
     float2 part[kFewRanges];
+#pragma unroll
+    for (int r = 0; r < kFewRanges; ++r) {
+      part[r] = make_float2(-INFINITY, 0.0f);
+      if (static_cast<uint32_t>(r) < all) part[r] = a.part[r * step + base];
+    }
+    const RowRanges ranges(a, kvh, row, length_of(a, row / a.seq_rows));
+    seen = ranges.seen;
     float top = -INFINITY;
-    whole.y = 0.0f;
 #pragma unroll
-    for (int r = 0; r < kFewRanges; ++r)
-      part[r] = static_cast<uint32_t>(r) < ranges.count() ? a.part[ranges.place(r)] : make_float2(-INFINITY, 0.0f);
-#pragma unroll
-    for (int r = 0; r < kFewRanges; ++r) top = fmaxf(top, part[r].x);
-    whole.x = reference_of(top);
+    for (int r = 0; r < kFewRanges; ++r) {
+      if (static_cast<uint32_t>(r) >= ranges.count()) part[r] = make_float2(-INFINITY, 0.0f);
+      top = fmaxf(top, part[r].x);
+    }
+    whole = make_float2(reference_of(top), 0.0f);
 #pragma unroll
     for (int r = 0; r < kFewRanges; ++r) {
       const float share = exp2_of(part[r].x - whole.x);
       whole.y = fma_rn(share, part[r].y, whole.y);
-      if (r % kAtOnce == static_cast<int>(first) && static_cast<uint32_t>(r) < ranges.count() && f < a.pitch) add(share, ranges.place(r));
+      if (r % kAtOnce == static_cast<int>(first) && static_cast<uint32_t>(r) < ranges.count()) add(share, ahead[r / kAtOnce]);
     }
   } else {
+    const RowRanges ranges(a, kvh, row, length_of(a, row / a.seq_rows));
+    seen = ranges.seen;
     whole = ranges.whole(a.part);
-    if (f < a.pitch) {
-#pragma unroll 4
-      for (uint32_t r = first; r < ranges.count(); r += kAtOnce) {
-        const uint64_t at = ranges.place(r);
-        add(exp2_of(a.part[at].x - whole.x), at);
-      }
+    auto share = [&](uint32_t r) { return exp2_of(a.part[r * step + base].x - whole.x); };
+#pragma unroll
+    for (int m = 0; m < kAhead; ++m) {
+      const uint32_t r = m * kAtOnce + first;
+      if (r < ranges.count()) add(share(r), ahead[m]);
     }
+#pragma unroll 4
+    for (uint32_t r = kAhead * kAtOnce + first; r < ranges.count(); r += kAtOnce)
+      add(share(r), *reinterpret_cast<const f32x4*>(sums + (r * step + base) * a.pitch));
   }
 #pragma unroll
   for (int off = kLanes; off < 64; off *= 2)
@@ -855,10 +878,10 @@ __device__ __forceinline__ void join_row(const Args& a, uint32_t task, f32x4 (*r
 #pragma unroll
     for (int w = 1; w < W; ++w) acc = acc + room[w][lane];
   }
-  if (lane == 0) a.whole[ranges.base] = make_float2(whole.x, 1.0f / whole.y);
+  if (lane == 0) a.whole[base] = make_float2(whole.x, 1.0f / whole.y);
   if (lane >= kLanes) return;
   T* out = static_cast<T*>(a.out) + query_offset(a, row, kvh);
-  const bool none = a.prefix + ranges.seen == 0;
+  const bool none = a.prefix + seen == 0;
   struct alignas(4 * sizeof(T)) Four {
     T v[4];
   } four;
