@@ -7,6 +7,8 @@
 // over the prefix's keys and, for new row i of a sequence that holds n rows,
 // its own keys j < n - rows + i + 1.  A row without a key is zeros.  A key
 // that a row does not see has no effect on it, whatever the key's bytes are.
+// Outputs are divided by their sum at the end and the maximum lags by at most
+// 2^13, so values below 2^114 / keys cannot overflow before that.
 //
 // Split.  All rows of a KV head (every sequence's, every new row's, the heads
 // of the group) are one matrix against the prefix, so the prefix is read once
@@ -800,10 +802,10 @@ struct RowRanges {
 constexpr int kFewRanges = 8;
 
 // Joins the ranges of one row (4 us where there are few rows, most of it launch
-// and the wait for the first loads; 12 us for 16,384 rows of four ranges, 34
-// MB).  D / 4 lanes hold a row of a range, four
-// features each, so a wavefront reads 256 / D ranges at a time and a workgroup
-// of W = 4 four times as many: the loads of a row are a few deep.
+// and the wait for the first loads; 14 us for 16,384 rows of four ranges, 34
+// MB).  D / 4 lanes hold a row of a range, four features each, so a wavefront
+// reads 256 / D ranges at a time and a workgroup of W = 4 four times as many:
+// the loads of a row are a few deep.
 template <class T, int D, int W>
 __device__ __forceinline__ void join_row(const Args& a, uint32_t task, f32x4 (*room)[64]) {
   constexpr int kLanes = D / 4, kAtOnce = W * 64 / kLanes;
@@ -946,9 +948,11 @@ __global__ __launch_bounds__(kThreads) void k_join(const Args a, uint32_t join_b
 
 // Weights of more rows: the scores again, a workgroup per 16 NT keys, held in
 // registers (2048 rows over 4096 keys, 8 KV heads: 42 us, 8 of products; the
-// query loads cost 15, the exponentials 2).  The wavefronts walk every fourth tile of the rows that see them;
-// a lane sums its keys over its rows, then the lanes and the wavefronts add up
-// in a fixed order.  Every key has one owner: no atomics.
+// query loads cost 15, the exponentials 2).  The wavefronts walk every fourth
+// tile of the rows that see them; a lane sums its keys over its rows, then the
+// lanes and the wavefronts add up in a fixed order.  Every key has one owner:
+// no atomics.  NT = 8 halves the query loads but leaves one workgroup to a
+// compute unit: 35 us at this size, but 34 instead of 24 over 2048 keys.
 template <class T, int D, Access A>
 __global__ __launch_bounds__(kThreads) void k_weights(const Args a) {
   using Ops = Operands<T, D, A>;

@@ -239,7 +239,8 @@ typedef struct dl_batch_shape {
  * j < length - rows + i + 1.  A row that sees no key is zeros; a key that a
  * row does not see has no effect on it, infinities and NaN included.  Widths
  * up to 256.  The prefix may be empty (its pointers null).  `scale` is a
- * device word, as dl_attention's. */
+ * device word, as dl_attention's.  The division by the sum comes last: finite
+ * values above 2^114 / keys may give infinities. */
 int dl_attention_shared_bytes(const dl_batch_shape* shape, uint64_t prefix, uint64_t* bytes);
 int dl_attention_shared(dl_queue* queue, int dtype, const dl_batch_shape* shape, const void* query,
                         const void* prefix_key, const void* prefix_value, uint64_t prefix, const void* key,
