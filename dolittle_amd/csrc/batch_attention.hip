@@ -761,7 +761,7 @@ void k_ranges(const Args a) {
   range.first = b * a.seq_rows + first;
   range.scores = a.scores ? a.scores + ((static_cast<uint64_t>(b) * a.kv_heads + range.kvh) * a.seq_rows + first) * a.score_pitch : nullptr;
   const uint64_t stride = static_cast<uint64_t>(a.kv_heads) * a.width;
-  const uint64_t at = (b * a.capacity * stride + static_cast<uint64_t>(range.kvh) * a.width) * sizeof(T);
+  const uint64_t at = (static_cast<uint64_t>(b) * a.capacity * stride + static_cast<uint64_t>(range.kvh) * a.width) * sizeof(T);
   range.keys = static_cast<const char*>(a.key) + at;
   range.values = static_cast<const char*>(a.value) + at;
   run_range<T, D, O, A, P>(a, range, shares, limit);
