@@ -327,9 +327,9 @@ struct Rows {
   static __device__ __forceinline__ int feature(int g, int j, int r) { return Across ? 16 * j + 4 * g + r : (4 * g + r) * C + j; }
 
   // Scores of the step at key `at` to exponentials against the maximum so far.
-  // A step whose exponentials sum to more than 2^13 in some lane (its scores
-  // pass that maximum by as much), and the first, raise the maximum and rescale
-  // what is summed; the others need no maximum of their own.
+  // A row whose exponentials of a step sum to more than 2^13 in some lane (its
+  // scores pass that maximum by as much), and that of a first step, raises its
+  // maximum and rescales what is summed; other steps need no maximum of their own.
   __device__ __forceinline__ void soften(f32x4 (&p)[QT][kTiles], bool masked, uint32_t at, float factor) {
     const int g = threadIdx.x % 64 / 16;
 #pragma unroll
@@ -355,11 +355,13 @@ struct Rows {
       };
       float s = weigh();
       if (rare(__any(!(s <= most[t])))) {
+        // Each row by itself: what another row sees changes no bit of this one.
+        const bool rises = group_max(s <= most[t] ? 0.0f : 1.0f) > 0.0f;
         if (masked) hide(p[t], -INFINITY);
         float high = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kTiles; ++u) high = fmaxf(high, fmaxf(fmaxf(p[t][u][0], p[t][u][1]), fmaxf(p[t][u][2], p[t][u][3])));
-        const float raised = fmaxf(top[t], group_max(high) * factor);
+        const float highest = group_max(high) * factor, raised = rises ? fmaxf(top[t], highest) : top[t];
         const float less = top[t] == -INFINITY ? 1.0f : exp2_of(top[t] - raised);  // nothing summed yet: zeros
         top[t] = raised;
         from[t] = -reference_of(raised);
