@@ -8,7 +8,7 @@ import pytest
 import batch_reference as ref
 from dolittle_amd import _lib
 from dolittle_amd.batch import BatchShape, workspace_bytes
-from test_gpu_batch import Problem, stored, value_of
+from test_gpu_batch import CODE, Problem, stored, up, value_of
 
 pytestmark = pytest.mark.gpu
 
@@ -56,11 +56,83 @@ forms = pytest.mark.parametrize("batch,rows,prefix,capacity,heads,lengths", FORM
 types = pytest.mark.parametrize("dtype", ["bf16", "f32"])
 
 
+@types
+@forms
+def test_maxima_that_rise_in_many_steps(device, queue, oracle, dtype, batch, rows, prefix, capacity, heads, lengths):
+    """Keys that grow along the sources: scores of some hundreds, most rows' maximum in a late step, and what
+    was summed before it is scaled down more than once."""
+    p = Problem(oracle, dtype, batch, rows, prefix, capacity, heads, lengths, spread=4.0)
+    grow = lambda k, axis: stored(oracle, value_of(k) * np.linspace(0.1, 2.0, k.shape[axis]).reshape(  # noqa: E731
+        [-1 if a == axis else 1 for a in range(k.ndim)]), dtype)
+    p.pk = grow(p.pk, 0)
+    for b, n in enumerate(lengths):
+        p.k[b, :n] = grow(p.k[b, :n], 0)
+    p.check(device, queue)
+
+
+@types
+@forms
+@pytest.mark.parametrize("scale", [-0.11, 0.0])
+def test_scales(device, queue, oracle, dtype, batch, rows, prefix, capacity, heads, lengths, scale):
+    p = Problem(oracle, dtype, batch, rows, prefix, capacity, heads, lengths)
+    p.scale = np.float32(scale)
+    p.check(device, queue)
+
+
+@types
+@forms
+def test_zero_scale_with_an_infinite_key(device, queue, oracle, dtype, batch, rows, prefix, capacity, heads, lengths):
+    """0 * inf is NaN for the last new row, which sees the key, and nothing to the others."""
+    p = Problem(oracle, dtype, batch, rows, prefix, capacity, heads, lengths)
+    p.scale = np.float32(0.0)
+    clean, _ = p.run(device, queue)
+    for b, n in enumerate(lengths):
+        p.k[b, n - 1] = stored(oracle, np.full(heads[2], np.inf), dtype)
+    got, weights = p.run(device, queue)
+    assert same_bits(got[:, :-1], clean[:, :-1])
+    assert np.all(np.isnan(value_of(got[:, -1])))
+    for b, n in enumerate(lengths):
+        assert np.all(np.isnan(weights[b, :, :n])) and np.all(weights[b, :, n:] == -7.0)
+
+
 def special_feature(oracle, dtype, rows, feature, value):
     """Those rows with one feature replaced."""
     rows = rows.copy()
     rows[..., feature] = stored(oracle, np.float32([value]), dtype)[0]
     return rows
+
+
+@types
+@forms
+@pytest.mark.parametrize("special", [np.inf, -np.inf, np.nan])
+def test_special_values_stay_in_their_feature(device, queue, oracle, dtype, batch, rows, prefix, capacity, heads, lengths,
+                                              special):
+    """One feature of the values of the last new rows, and of a late prefix row, is not finite: it reaches that
+    feature of the rows that see it, and no other bit changes."""
+    width, late = heads[2], min(rows, 2)
+    p = Problem(oracle, dtype, batch, rows, prefix, capacity, heads, lengths)
+    clean, clean_weights = p.run(device, queue)
+    values, prefix_values = p.v, p.pv
+    for feature in (0, width // 2 + 3, width - 1):
+        others = np.arange(width) != feature
+        p.v = values.copy()
+        for b, n in enumerate(lengths):  # seen by the last `late` rows
+            p.v[b, n - late] = special_feature(oracle, dtype, values[b, n - late], feature, special)
+        got, weights = p.run(device, queue)
+        assert same_bits(got[..., others], clean[..., others])
+        assert same_bits(got[:, :rows - late], clean[:, :rows - late])
+        assert np.array_equal(value_of(got[:, rows - late:, :, feature]),
+                              np.full((batch, late, heads[0]), special), equal_nan=True)
+        assert same_bits(weights, clean_weights)
+        p.v, p.pv = values, prefix_values.copy()
+        if not prefix:
+            continue
+        p.pv[prefix - 2] = special_feature(oracle, dtype, p.pv[prefix - 2], feature, special)
+        got, weights = p.run(device, queue)
+        assert same_bits(got[..., others], clean[..., others])
+        assert np.array_equal(value_of(got[..., feature]), np.full((batch, rows, heads[0]), special), equal_nan=True)
+        assert same_bits(weights, clean_weights)
+        p.pv = prefix_values
 
 
 @types
@@ -107,3 +179,65 @@ def test_special_keys(device, queue, oracle, dtype, batch, rows, prefix, capacit
         wide = first_bound[b][:, rest] + last_bound[b][:, :n - 1] + 2.0 ** -23 * np.abs(total)
         wide += added * (rows * heads[0] // heads[1]) * 2.0 ** -24  # a rounding for each row and head added
         assert np.all(np.abs(weights[b][:, rest] - total) <= wide)
+
+
+@types
+@pytest.mark.parametrize("batch,rows,prefix,capacity,heads,lengths", [
+    (9, 1, 1000, 4096, (8, 2, 128), [5, 4, 3, 2, 1, 0, 5, 300, 5]),
+    (2, 1, 3000, 20000, (8, 2, 64), [200, 31]),
+    (2, 20, 700, 9000, (8, 2, 128), [150, 40]),
+    (1, 66, 8100, 5000, (8, 8, 128), [69]),
+    (3, 16, 1001, 8192, (8, 2, 128), [115, 16, 40]),
+    (1, 1, 0, 1 << 20, (2, 1, 8), [129]),
+])
+def test_caches_with_room_left(device, queue, oracle, dtype, batch, rows, prefix, capacity, heads, lengths):
+    """Caches of many more slots than rows in use, as a program allocates them: ranges and the join go by the slots."""
+    Problem(oracle, dtype, batch, rows, prefix, capacity, heads, lengths).check(device, queue)
+
+
+@types
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("apart", range(6))
+def test_attention_with_one_operand_off_alignment(device, queue, oracle, dtype, rows, apart):
+    """An element past an aligned address for one of the query, the prefix, the cache and the output."""
+    p = Problem(oracle, dtype, 2, rows, 40, 90, (8, 2, 128), [90, 41])
+    out, bound, _, _ = p.want()
+    at = [up(device, queue, x, int(i == apart)) for i, x in enumerate((p.q, p.pk, p.pv, p.k, p.v, np.zeros_like(p.q)))]
+    lengths, scale = up(device, queue, p.lengths), up(device, queue, np.array([p.scale]))
+    room = workspace_bytes("dl_attention_shared", p.shape, p.prefix)
+    work = device.allocate(room)
+    _lib.call("dl_attention_shared", queue.handle, CODE[dtype], C.byref(p.shape), *[x[1] for x in at[:3]], p.prefix, at[3][1],
+              at[4][1], lengths[1], at[5][1], scale[1], work.ptr(), room)
+    raw = queue.read(at[5][0], p.q.dtype, p.q.size + int(apart == 5) + 1)
+    assert raw[-1] == 0 and (apart < 5 or raw[0] == 0)  # what lies beside the output stays
+    got = raw[int(apart == 5):-1].reshape(p.q.shape)
+    assert np.all(np.abs(value_of(got) - out) <= bound)
+
+
+@types
+@pytest.mark.parametrize("width", [64, 128, 12])
+@pytest.mark.parametrize("apart", ["q", "k", "v", "q2", "keys", "values"])
+def test_append_with_one_operand_off_alignment(device, queue, oracle, dtype, width, apart):
+    """The bits of the aligned call, whichever operand lies an element past an aligned address."""
+    batch, rows, capacity, qh, kvh = 2, 3, 11, 6, 2
+    rng = np.random.default_rng(width)
+    make = lambda *s: stored(oracle, rng.standard_normal(s), dtype)  # noqa: E731
+    a = dict(q=make(batch, rows, qh, width), k=make(batch, rows, kvh, width), v=make(batch, rows, kvh, width))
+    a.update(q2=np.zeros_like(a["q"]), keys=make(batch, capacity, kvh, width), values=make(batch, capacity, kvh, width),
+             lengths=np.array([3, 9], np.uint64), lengths2=np.zeros(2, np.uint64), positions=np.array([70, 9], np.uint64),
+             positions2=np.zeros(2, np.uint64), slots=np.zeros((batch, kvh, capacity), np.uint32),
+             weights=np.ones((batch, kvh, capacity), np.float32))
+
+    def run(off):
+        b = {n: up(device, queue, x, int(n == off)) for n, x in a.items()}
+        shape = BatchShape(batch, rows, qh, kvh, width, capacity)
+        _lib.call("dl_cache_append", queue.handle, CODE[dtype], C.byref(shape), *[x[1] for x in b.values()], 1e6)
+        whole = {n: queue.read(b[n][0], x.dtype, x.size + int(n == off) + 1) for n, x in a.items()}
+        for n, x in whole.items():  # what lies beside an operand stays
+            assert x[-1] == 0 and (n != off or x[0] == 0)
+        return {n: x[int(n == off):-1] for n, x in whole.items()}
+
+    want, got = run(None), run(apart)
+    assert not np.array_equal(want["keys"], a["keys"].reshape(-1)) and np.any(want["q2"])
+    for n in a:
+        assert same_bits(got[n], want[n]), n
