@@ -249,7 +249,7 @@ struct Args {
   void* out;
   float2* part;  // [ranges][kv head][row]: maximum, sum
   float* sums;   // [ranges][kv head][row][pitch]: unnormalised output
-  float2* whole; // [kv head][row]: maximum, 1 / sum
+  float2* whole; // [kv head][row]: maximum, 1 / sum, for k_weights, or null
   float* scores; // [batch][kv head][seq row][score_pitch]: own scores before the scale, or null
   const float* weights;
   float* weights_out;
@@ -882,7 +882,7 @@ __device__ __forceinline__ void join_row(const Args& a, uint32_t task, f32x4 (*r
 #pragma unroll
     for (int w = 1; w < W; ++w) acc = acc + room[w][lane];
   }
-  if (lane == 0) a.whole[base] = make_float2(whole.x, 1.0f / whole.y);
+  if (a.whole && lane == 0) a.whole[base] = make_float2(whole.x, 1.0f / whole.y);
   if (lane >= kLanes) return;
   T* out = static_cast<T*>(a.out) + query_offset(a, row, kvh);
   const bool none = a.prefix + seen == 0;
@@ -1164,7 +1164,7 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted, bo
   const uint64_t entries = product({uint64_t{a.prefix_splits} + a.own_splits, a.kv_heads, a.all_rows}, kMost, kLarge);
   l.part_bytes = room({entries, 8});
   l.sums_bytes = room({entries, a.pitch, 4});
-  l.whole_bytes = room({a.kv_heads, a.all_rows, 8});
+  l.whole_bytes = weighted && !l.stored ? room({a.kv_heads, a.all_rows, 8}) : 0;
   l.score_bytes = l.stored ? room({a.kv_heads, a.all_rows, a.score_pitch, 4}) : 0;
   return l;
 }
@@ -1267,8 +1267,9 @@ void submit(dl_queue* queue, int dtype, const dl_batch_shape* shape, uint64_t pr
   char* room = static_cast<char*>(o.workspace);
   a.part = reinterpret_cast<float2*>(room);
   a.sums = reinterpret_cast<float*>(room + l.part_bytes);
-  a.whole = reinterpret_cast<float2*>(room + l.part_bytes + l.sums_bytes);
-  if (l.stored) a.scores = reinterpret_cast<float*>(room + l.part_bytes + l.sums_bytes + l.whole_bytes);
+  char* for_weights = room + l.part_bytes + l.sums_bytes;
+  if (l.whole_bytes) a.whole = reinterpret_cast<float2*>(for_weights);
+  if (l.score_bytes) a.scores = reinterpret_cast<float*>(for_weights);
   a.weights = static_cast<const float*>(o.weights);
   a.weights_out = o.weights_out;
   if (dtype == DL_BF16)

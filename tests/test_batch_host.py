@@ -117,6 +117,19 @@ def test_workspace_covers_what_is_written():
     assert weighted - plain >= 4 * rows * 8
 
 
+def test_workspace_of_the_weights():
+    """The weights of up to 16 rows a KV head need their scores, those of more rows each row's maximum and sum;
+    the attention alone needs neither."""
+    def pieces(nbytes):
+        return (nbytes + 255) // 256 * 256
+
+    for rows, heads, extra in ((5, 3, lambda s: s.rows * 704 * 4), (16, 1, lambda s: s.rows * 704 * 4),
+                               (6, 3, lambda s: s.rows * 8), (17, 1, lambda s: s.rows * 8)):
+        s = shape(batch=3, rows=rows, query_heads=4 * heads, kv_heads=4, width=80, capacity=700)
+        plain, weighted = (workspace_bytes(n, s, 1000) for n in NAMES)
+        assert weighted - plain == pieces(extra(s) * 3 * 4 * heads), (rows, heads)
+
+
 def test_append_refusals():
     for i in range(12):
         with pytest.raises(InvalidArgument, match="null operand"):
