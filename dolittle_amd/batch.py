@@ -90,8 +90,9 @@ class BatchCache:
                   room)
 
     def evict(self, budget: int, sinks: int = 0, recent: int = 0) -> None:
-        """Cuts every sequence to at most `budget` rows, keeping the first `sinks` positions, the last `recent`
-        and then the rows that received most attention."""
+        """Cuts every sequence to at most `budget` rows, keeping those at a position below `sinks`, the last `recent`
+        and then the rows that received most attention.  Positions count from the sequence's start: behind a prefix
+        of `sinks` or more positions, which holds those rows and is never cut, no own row is a sink."""
         if budget <= 0 or sinks < 0 or recent < 0:
             raise _lib.InvalidArgument("invalid eviction budget")
         shape = self.shape()

@@ -270,13 +270,16 @@ int dl_cache_append(dl_queue* queue, int dtype, const dl_batch_shape* shape, con
 /* Cuts every sequence that holds more than `budget` rows to `budget`, per KV
  * head: rows at a position below `sinks` or within `recent` of the head's
  * newest position stay, then those of the largest weight (NaN as -infinity,
- * equal weights by the lower slot).  sinks + recent must not exceed budget
- * (head positions are distinct).  In place, moving the fewest rows: the j-th
- * slot below the budget whose row does not stay takes the j-th row at or above
- * it that does; attention does not depend on the order, and `slots` says which
- * position a slot holds.  slots_out, weights_out and lengths_out may be their
- * inputs; their entries past the new length are left as they were.  The
- * shape's rows and query_heads are not used. */
+ * equal weights by the lower slot).  `sinks` counts positions from the
+ * sequence's start, not slots: own rows behind a shared prefix of that many
+ * positions are not sinks (the prefix holds those, and is never cut).  sinks +
+ * recent must not exceed budget (head positions are distinct).  In place,
+ * moving the fewest rows: the j-th slot below the budget whose row does not
+ * stay takes the j-th row at or above it that does; attention does not depend
+ * on the order, and `slots` says which position a slot holds.  slots_out,
+ * weights_out and lengths_out may be their inputs; their entries past the new
+ * length are left as they were.  The shape's rows and query_heads are not
+ * used. */
 int dl_cache_evict_bytes(const dl_batch_shape* shape, uint64_t budget, uint64_t* bytes);
 int dl_cache_evict(dl_queue* queue, int dtype, const dl_batch_shape* shape, void* keys, void* values,
                    const uint64_t* lengths, uint64_t* lengths_out, const uint32_t* slots, uint32_t* slots_out,

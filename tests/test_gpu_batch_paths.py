@@ -7,7 +7,7 @@ import pytest
 
 import batch_reference as ref
 from dolittle_amd import _lib
-from dolittle_amd.batch import BatchShape, workspace_bytes
+from dolittle_amd.batch import BatchCache, BatchShape, workspace_bytes
 from test_gpu_batch import CODE, Problem, stored, up, value_of
 
 pytestmark = pytest.mark.gpu
@@ -241,3 +241,20 @@ def test_append_with_one_operand_off_alignment(device, queue, oracle, dtype, wid
     assert not np.array_equal(want["keys"], a["keys"].reshape(-1)) and np.any(want["q2"])
     for n in a:
         assert same_bits(got[n], want[n]), n
+
+
+# ------------------------------------------------------------ the cache object
+@pytest.mark.parametrize("first", [0, 3])
+def test_sinks_are_positions_of_the_sequence(device, queue, oracle, first):
+    """`sinks` counts positions from the sequence's start: rows behind a prefix that holds them all are not sinks."""
+    rows, budget, width = 10, 8, 8
+    for sinks in (first, first + 2):
+        cache = BatchCache(device, queue, 1, rows, 1, 1, width, first_position=first)
+        q, k, v = (device.upload_array(queue, np.zeros(rows * width, np.uint16)) for _ in range(3))
+        cache.append(q, k, v, q, rows)
+        queue.write(cache.weights, np.arange(rows, dtype=np.float32))  # the first rows received least
+        cache.evict(budget, sinks)
+        slots = queue.read(cache.slots, np.uint32, rows)[:budget]
+        gone = {first, first + 1} if sinks == first else {first + 2, first + 3}
+        assert set(slots.tolist()) == set(range(first, first + rows)) - gone
+        assert cache.used == [budget]
