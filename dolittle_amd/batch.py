@@ -36,8 +36,9 @@ class BatchCache:
     that need no device value), so a row that does not fit is refused here.
     Every method only enqueues, except that a first attend or evict that needs
     more workspace allocates it: run a step once before it is recorded into a
-    graph, and add a replayed step's rows to `used`.  `query` and the rows are
-    device addresses or buffers, [batch][rows][heads][width].
+    graph.  Recording a step counts its rows in `used` once; add those of every
+    replay after the first.  `query` and the rows are device addresses or
+    buffers, [batch][rows][heads][width].
     """
 
     def __init__(self, device: Device, queue: Queue, batch: int, capacity: int, query_heads: int, kv_heads: int,

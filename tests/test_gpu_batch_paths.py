@@ -258,3 +258,41 @@ def test_sinks_are_positions_of_the_sequence(device, queue, oracle, first):
         gone = {first, first + 1} if sinks == first else {first + 2, first + 3}
         assert set(slots.tolist()) == set(range(first, first + rows)) - gone
         assert cache.used == [budget]
+
+
+def test_used_counts_a_recorded_step_once(device, queue, oracle):
+    """A step recorded through the object counts as one replay; the program adds the rows of the others."""
+    batch, capacity, prefix, qh, kvh, w, replays = 2, 9, 20, 4, 2, 64, 4
+    rng = np.random.default_rng(8)
+    make = lambda *s: up(device, queue, stored(oracle, rng.standard_normal(s), "bf16"))[0]  # noqa: E731
+    cache = BatchCache(device, queue, batch, capacity, qh, kvh, w, first_position=prefix)
+    cache.set_prefix(make(prefix, kvh, w), make(prefix, kvh, w), prefix)
+    q, k, v = make(batch, 1, qh, w), make(batch, 1, kvh, w), make(batch, 1, kvh, w)
+    turned, out = device.allocate(batch * qh * w * 2), device.allocate(batch * qh * w * 2)
+
+    def step():
+        cache.append(q, k, v, turned)
+        cache.attend(turned, out)
+
+    step()  # allocates the workspace
+    ids = device.upload_array(queue, np.arange(replays, dtype=np.uint32))
+    token = device.allocate(4)
+    handle = C.c_void_p()
+    _lib.call("dl_sequence_create", queue.handle, replays, 0, 1, 1, C.byref(handle))
+    try:
+        _lib.call("dl_sequence_begin", handle, None, None, token.ptr(), 4, ids.ptr(), replays * 4, None, None, None, None)
+        for stage in range(4):
+            _lib.call("dl_sequence_begin_stage", handle, stage)
+            if stage == 0:
+                step()
+            if stage == 3:
+                _lib.call("dl_sequence_begin_selection", handle)
+            _lib.call("dl_sequence_end_stage", handle)
+        _lib.call("dl_sequence_complete", handle)
+        _lib.call("dl_sequence_start", handle)
+        _lib.call("dl_sequence_drain", handle)
+    finally:
+        _lib.call("dl_sequence_destroy", handle)
+    cache.used = [n + replays - 1 for n in cache.used]
+    assert cache.used == [int(n) for n in queue.read(cache.lengths, np.uint64, batch)] == [1 + replays] * batch
+    assert list(queue.read(cache.positions, np.uint64, batch)) == [prefix + 1 + replays] * batch
