@@ -486,8 +486,11 @@ __device__ __forceinline__ void run_apart(const Args& a, const Range& range, Row
       load_words<T, C, A>(base, min(value_offset + Ops::value_key(0, r) * stride, most), i16 * C, width, vf.v[r]);
   };
   // Steps past the range repeat its last key: operands are defined on every
-  // path.  (With the loads under a condition the compiler has reused part of
-  // a loaded row's registers before its last use.)
+  // path.  (With these loads under `next < end`, which leaves no use undefined
+  // either, hipcc of ROCm 7.2 assembles value operands in the registers of the
+  // first loaded row, whose other words are read later: wrong results from the
+  // BF16 kernels of 128 and 256 features.  tests/test_batch_code.py looks for
+  // that in the built code.)
   uint32_t at = range.begin + wave * KT;
   if (at < end) {
     load_keys(at);
