@@ -8,7 +8,7 @@ import pytest
 import batch_reference as ref
 from dolittle_amd import _lib
 from dolittle_amd.batch import BatchCache, BatchShape, workspace_bytes
-from test_gpu_batch import CODE, Problem, stored, up, value_of
+from test_gpu_batch import CODE, Problem, evict_inputs, stored, up, value_of, want_evict
 
 pytestmark = pytest.mark.gpu
 
@@ -241,6 +241,30 @@ def test_append_with_one_operand_off_alignment(device, queue, oracle, dtype, wid
     assert not np.array_equal(want["keys"], a["keys"].reshape(-1)) and np.any(want["q2"])
     for n in a:
         assert same_bits(got[n], want[n]), n
+
+
+@types
+@pytest.mark.parametrize("width", [128, 12])
+@pytest.mark.parametrize("apart", ["keys", "values"])
+def test_evict_with_one_operand_off_alignment(device, queue, oracle, dtype, width, apart):
+    batch, capacity, kvh, budget = 2, 90, 2, 41
+    k, v, weights, slots = evict_inputs(oracle, dtype, batch, kvh, width, capacity, width)
+    lengths = np.array([90, 60], np.uint64)
+    shape = BatchShape(batch, 1, kvh, kvh, width, capacity)
+    b = [up(device, queue, x, int(n == apart)) for n, x in (("keys", k), ("values", v))]
+    n, w, at = (up(device, queue, x) for x in (lengths, weights, slots))
+    room = workspace_bytes("dl_cache_evict", shape, budget)
+    work = device.allocate(room)
+    _lib.call("dl_cache_evict", queue.handle, CODE[dtype], C.byref(shape), b[0][1], b[1][1], n[1], n[1], at[1], at[1], w[1], w[1],
+              budget, 2, 9, work.ptr(), room)
+    want = want_evict(k, v, weights, slots, lengths, budget, 2, 9, True)
+    for name, buf, e in zip(("keys", "values"), b, want):
+        off = int(name == apart)
+        raw = queue.read(buf[0], e.dtype, e.size + off + 1)
+        assert raw[-1] == 0 and (not off or raw[0] == 0)
+        assert same_bits(raw[off:-1], e.reshape(-1)), name
+    for buf, e in zip((w, at, n), want[2:]):
+        assert same_bits(queue.read(buf[0], e.dtype, e.size), e.reshape(-1))
 
 
 # ------------------------------------------------------------ the cache object
