@@ -10,7 +10,8 @@
 namespace dl::batch {
 
 // Most keys of a prefix or cache, and most elements of one key row over all KV
-// heads: a step of 32 rows is addressed with 32-bit offsets from a 64-bit base.
+// heads: up to 64 rows (the last one's offset at most 63 * 2^26 + 2^10 bytes)
+// are addressed with 32-bit offsets from a 64-bit base.
 constexpr uint64_t kMostKeys = 1u << 30;
 constexpr uint64_t kMostRow = 1u << 24;
 

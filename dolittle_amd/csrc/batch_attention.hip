@@ -25,21 +25,25 @@
 // P^T operand of V^T P^T wants from it; a lane loads C = D / 16 neighbouring
 // features of each of its keys, and since any 16 features may form a matrix
 // tile, tile j takes feature j of every lane's C: the transposition is a byte
-// permute (BF16) or nothing (FP32).  Bound by the key and value stream: 8
-// sequences of up to 4607 keys, 101 MB in 26 us, of which 4 until the first
-// step has landed (6.15 TB/s is this card's rate for a large read).  FP32 is
-// bound by its matrix rate: 48 rows a KV head over 1001 keys 19 us, 6 at 154
-// TFLOP/s; what is more is the first loads and two workgroups to a compute unit.
+// permute (BF16) or nothing (FP32).  Bound by the key and value stream with one
+// step in flight a wavefront: 8 sequences of up to 4607 keys, 101 MB in 26 us,
+// of which 4 until the first step has landed (6.15 TB/s is this card's rate for
+// a large read).  FP32, 192 rows a KV head over 1001 keys: 19 us, 6 at 154
+// TFLOP/s; the matrix unit is busy 34% of the time, and wavefronts, two to a
+// SIMD, wait 57% of theirs for an instruction to issue and 29% for loads.
 //
 // More BF16 rows run together: 16 or 32 in each wavefront, keys and values
 // through LDS for all four (64 sequences over 32768 keys 84 us, 114 with every
-// wavefront loading its own).  Bound by the issue of vector instructions beside
-// the matrix products, two wavefronts to a SIMD: a step of 32 rows and 32 keys
-// takes about 1050 cycles, 512 of them products (512 rows of 4 heads over 4096
-// keys 52 us, 630 TFLOP/s).  Which form is taken goes by rows and storage
-// alone; 128 rows a workgroup instead of 64 where those still fill the chip.
+// wavefront loading its own).  Bound by the chain of one step, products, softmax
+// and products again, with fewer than two wavefronts to a SIMD to fill it: 512
+// rows of 4 heads over 4096 keys 54 us, 600 TFLOP/s, products 30% of a SIMD's
+// cycles and vector instructions 45%; 64 sequences 21% and 31%.  Which form is
+// taken goes by rows and storage alone; 128 rows a workgroup instead of 64 where
+// those still fill the chip.
 //
-// BF16 storage rounds P to BF16 (8 bits, relative 2^-9) for the product with V;
+// BF16 storage rounds P to BF16 (8 bits, off by at most 2^-8 of the value) for the
+// product with V, as BF16 matrix operands need: 0.20 to 0.23% off 64-bit results
+// where rounding the output alone is 0.17%;
 // scores, exponentials, sums, maxima and outputs are FP32 throughout, and so
 // are the weights.  FP32 storage runs FP32 matrix instructions.
 #include <algorithm>
@@ -1147,7 +1151,11 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t prefix, bool weighted, bo
   const Mode own = mode_of(a.seq_rows, uint64_t{a.batch} * a.kv_heads * ceil_div(a.capacity, kRound));
   const Mode all = prefix ? mode_of(a.all_rows, a.kv_heads * ceil_div(prefix, kRound)) : own;
   l.set_modes(all, a.seq_rows <= 32 ? Mode::kApart : all);
-  // Ranges: as many workgroups as the chip holds at once, each with whole rounds of keys.
+  // Ranges: as many workgroups as the chip holds at once, each with whole rounds
+  // of keys.  Lengths lie on the device, so a cache counts with all its slots: the
+  // more of them are free, the fewer ranges are left for the prefix (64 sequences
+  // of up to 1000 rows over 32768 keys, caches of 1008 slots 88 us, 2008 106, 8008
+  // 224, 32008 814).
   const uint64_t held = 256 * (l.features == 256 ? 1 : l.features == 64 ? 3 : 2);
   const double work = static_cast<double>(a.kv_heads) *
                       (static_cast<double>(a.prefix_tiles) * a.prefix +
@@ -1180,7 +1188,7 @@ uint64_t workspace_of(const dl_batch_shape* shape, uint64_t prefix, bool weighte
 template <class T, int D, Access A>
 void launch(hipStream_t s, const Layout& l) {
   const Args& a = l.args;
-  const unsigned blocks = a.prefix_blocks + l.own_blocks;  // at most 2^31
+  const unsigned blocks = a.prefix_blocks + l.own_blocks;  // below 2^24: 2^32 threads
   auto run = [&](auto prefix, auto own) {
     k_ranges<T, D, decltype(prefix)::value, decltype(own)::value, A><<<blocks, kThreads, 0, s>>>(a);
   };

@@ -422,7 +422,8 @@ __global__ __launch_bounds__(Threads) void k_select(const EvictArgs a) {
 // copies those of the rows that stay.  Holes lie below the budget and their
 // sources at or above it, so no row is both read and written and the outputs
 // may be the inputs; no length is read, so neither need lengths_out differ.
-// Bound by the copy: 64 heads, 268 MB read and written, 55 us.
+// Bound by the copy: 64 heads, 268 MB read and written in 65 us, 4.1 TB/s (a
+// large copy reaches 4.9).
 template <class Piece>
 __global__ __launch_bounds__(256) void k_move(const EvictArgs a, uint32_t row_pieces) {
   const uint32_t head = blockIdx.y, b = head / a.kv_heads, h = head % a.kv_heads;
