@@ -136,6 +136,11 @@ class BatchShape(C.Structure):
                 ("width", C.c_uint64), ("capacity", C.c_uint64)]
 
 
+class Fp4Cache(C.Structure):
+    _fields_ = [("key_codes", C.c_void_p), ("key_scales", C.c_void_p), ("value_codes", C.c_void_p),
+                ("value_scales", C.c_void_p)]
+
+
 # name -> argument types (all return int status)
 SIGNATURES = {
     "dl_device_open": [cint, vpp],
@@ -180,6 +185,13 @@ SIGNATURES = {
     "dl_cache_append": [vp, cint, C.POINTER(BatchShape), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_double],
     "dl_cache_evict_bytes": [C.POINTER(BatchShape), u64, u64p],
     "dl_cache_evict": [vp, cint, C.POINTER(BatchShape), vp, vp, vp, vp, vp, vp, vp, vp, u64, u64, u64, vp, u64],
+    "dl_fp4_bytes": [u64, u64, u64p, u64p],
+    "dl_fp4_quantize": [vp, cint, vp, vp, vp, u64, u64],
+    "dl_fp4_values": [vp, cint, vp, vp, vp, u64, u64],
+    "dl_projection_fp4": [vp, cint, vp, vp, vp, vp, u64, u64, u64, vp],
+    "dl_cache_append_fp4": [vp, cint, C.POINTER(BatchShape), vp, vp, vp, vp, C.POINTER(Fp4Cache), vp, vp, vp, vp, C.c_double],
+    "dl_attention_fp4_bytes": [C.POINTER(BatchShape), u64, u64, u64p],
+    "dl_attention_fp4": [vp, cint, C.POINTER(BatchShape), vp, C.POINTER(Fp4Cache), vp, u64, u64, vp, vp, vp, u64],
     "dl_qwen3_create": [vp, vp, C.POINTER(Qwen3Config), vpp],
     "dl_qwen3_destroy": [vp],
     "dl_qwen3_fill_synthetic": [vp, vp, u64, C.c_float],

@@ -1,0 +1,87 @@
+// Rows held in 4 bits, shared by fp4.hip and fp4_attention.hip: groups of 32
+// values, each 16 bytes of codes (the lower half of a byte first) and one scale
+// byte s.  A code is a sign, two bits of exponent and one of fraction: 0, 0.5, 1,
+// 1.5, 2, 3, 4 or 6, times 2^(s - 127); s = 255 makes the whole group NaN.  This
+// is the OCP microscaling format MXFP4.  CDNA4 converts two codes under a scale
+// in one instruction, and their values are exact in BF16.
+#pragma once
+
+#include <cstdint>
+
+#include "dl_device.h"
+#include "dl_internal.h"
+
+namespace dl::fp4 {
+
+constexpr int kGroup = 32, kGroupBytes = 16;
+constexpr uint32_t kNanScale = 255;
+// Largest scale byte that quantising gives: 6 * 2^(252 - 127) is still finite.
+constexpr uint32_t kMostScale = 252;
+
+inline uint64_t groups_of(uint64_t width) { return ceil_div(width, kGroup); }
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// The conversions read a scale's exponent field alone: the scale byte's bits as
+// they are, 2^-127 among them, and NaN for 255.
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// Eight codes to eight BF16 values in order.
+__device__ __forceinline__ u32x4 to_bf16(uint32_t codes, float scale) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+}
+
+// FP32 values as the exact sum of three BF16 values each (8 significant bits at a
+// time), for products on the BF16 matrix cores that round nothing.  A value that
+// is not finite is its first part alone.
+struct Parts {
+  u32x4 part[3];
+};
+__device__ __forceinline__ Parts split(const float (&x)[8]) {
+  Parts p;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t high[2], middle[2], low[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float v = x[2 * w + e];
+      const bool finite = fabsf(v) < INFINITY;
+      high[e] = v == v ? __float_as_uint(v) & 0xffff0000u : 0x7fc00000u;
+      const float rest = finite ? v - __uint_as_float(high[e]) : 0.0f;
+      middle[e] = __float_as_uint(rest) & 0xffff0000u;
+      low[e] = __float_as_uint(rest - __uint_as_float(middle[e]));
+    }
+    p.part[0][w] = __builtin_amdgcn_perm(high[1], high[0], 0x07060302u);
+    p.part[1][w] = __builtin_amdgcn_perm(middle[1], middle[0], 0x07060302u);
+    p.part[2][w] = __builtin_amdgcn_perm(low[1], low[0], 0x07060302u);
+  }
+  return p;
+}
+
+// The scale byte of a group whose largest magnitude has these FP32 bits: the power
+// of two under which it lies in [3.5, 7), so that no value passes 6, the largest
+// code, by more than half of the step there; kNanScale if a value is not finite.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t largest) {
+  if (largest >= 0x7f800000u) return kNanScale;
+  const int32_t s = static_cast<int32_t>((largest + 0x200000u) >> 23) - 2;
+  return static_cast<uint32_t>(min(max(s, 0), static_cast<int32_t>(kMostScale)));
+}
+
+// Eight values to eight codes: to nearest, ties to the even code, 6 at most.
+__device__ __forceinline__ uint32_t to_codes(const float (&x)[8], uint32_t byte) {
+  if (byte == kNanScale) return 0;
+  const float by = scale_of(byte);
+  uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[0], x[1], by, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], by, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], by, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], by, 3);
+}
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+}  // namespace dl::fp4

@@ -290,6 +290,73 @@ int dl_cache_evict(dl_queue* queue, int dtype, const dl_batch_shape* shape, void
                    const float* weights, float* weights_out, uint64_t budget, uint64_t sinks, uint64_t recent,
                    void* workspace, uint64_t workspace_bytes);
 
+/* ------------------------------------- weights and caches held in 4 bits */
+/* Rows in groups of 32 values, each 16 bytes of codes and one scale byte.  No
+ * reference counterpart: the reference keeps weights and caches in BF16 or FP32.
+ * The format is the OCP microscaling format MXFP4: byte i of a group holds value
+ * 2 i in its lower half and 2 i + 1 in its upper; a code's bits are sign,
+ * exponent (2) and fraction (1), its magnitudes 0, 0.5, 1, 1.5, 2, 3, 4 and 6;
+ * scale byte s is the factor 2^(s - 127), and 255 makes the group NaN (253 and 254
+ * are never written and must not be read).  A row of `width` values has groups =
+ * ceil(width / 32); codes past the width are zeros.
+ *
+ *   weights          codes [outputs][groups][16], scales [outputs][groups]
+ *   caches           codes [batch][kv_heads][capacity][groups][16], scales
+ *                    [batch][kv_heads][capacity][groups]
+ *
+ * Codes are 16-byte aligned; scales and all other operands may be element-aligned
+ * and of any width; rows in 16-byte pieces run fastest.  dtype (DL_BF16 or DL_F32)
+ * is the storage of the other operands; sums are FP32, and FP32 storage rounds
+ * nothing to fewer bits.  Operands do not overlap except where an operation says
+ * that they may.  No operation allocates, waits, or uses atomics on results: the
+ * same call gives the same bits, and calls may be captured into graphs. */
+typedef struct dl_fp4_cache { /* device addresses */
+  void* key_codes;
+  void* key_scales;
+  void* value_codes;
+  void* value_scales;
+} dl_fp4_cache;
+
+/* Bytes of the codes and of the scales of `rows` rows. */
+int dl_fp4_bytes(uint64_t rows, uint64_t width, uint64_t* codes, uint64_t* scales);
+/* Quantises rows [rows][width].  A group's scale is the power of two under which
+ * its largest magnitude lies in [3.5, 7), but s is 0 to 252; values are rounded to
+ * the nearest code, ties to the even one, 6 at most.  A group with a value that is
+ * not finite becomes NaN. */
+int dl_fp4_quantize(dl_queue* queue, int dtype, const void* input, void* codes, void* scales, uint64_t rows,
+                    uint64_t width);
+/* The values that rows of codes and scales stand for, [rows][width]; exact in both
+ * types. */
+int dl_fp4_values(dl_queue* queue, int dtype, const void* codes, const void* scales, void* output, uint64_t rows,
+                  uint64_t width);
+/* dl_projection with 4-bit weights: Y[R,O] = X[R,I] W[O,I]^T, one rounding of the
+ * FP32 sum.  Fast for one to 16 rows, which read the weights once; a NaN group
+ * makes its output NaN. */
+int dl_projection_fp4(dl_queue* queue, int dtype, const void* input, const void* codes, const void* scales,
+                      void* output, uint64_t rows, uint64_t input_width, uint64_t output_width,
+                      const uint64_t* output_position);
+/* dl_cache_append to a cache held in 4 bits (no slots and weights: nothing is
+ * evicted from it).  Rotated keys go from FP32 to 4 bits in one rounding.  Rows
+ * past the capacity are dropped, the length stays at the capacity.  Head widths up
+ * to 256, even.  query_out may be query, lengths_out and positions_out their
+ * inputs. */
+int dl_cache_append_fp4(dl_queue* queue, int dtype, const dl_batch_shape* shape, const void* query, const void* key,
+                        const void* value, void* query_out, const dl_fp4_cache* cache, const uint64_t* lengths,
+                        uint64_t* lengths_out, const uint64_t* positions, uint64_t* positions_out, double theta);
+/* out = softmax(scale * Q K^T) V over each sequence's cache.  `lengths` includes
+ * the new rows, which are the last `rows`: new row i is at slot p = length - rows +
+ * i and sees slots j <= p; with a window (not 0) only those with j > p - window,
+ * and the first `sinks` slots up to p.  Rows out of sight are not read: a step costs
+ * by its window.  A row that sees no key is zeros; a key that a row does not see
+ * has no effect on it, NaN groups included.  Widths up to 256.  `scale` is a device
+ * word, as dl_attention's.  BF16 storage rounds every softmax weight to BF16 for its
+ * product with V.  The workspace (16-byte aligned; of no bytes it may be null)
+ * belongs to one call at a time; its contents need not survive. */
+int dl_attention_fp4_bytes(const dl_batch_shape* shape, uint64_t window, uint64_t sinks, uint64_t* bytes);
+int dl_attention_fp4(dl_queue* queue, int dtype, const dl_batch_shape* shape, const void* query,
+                     const dl_fp4_cache* cache, const uint64_t* lengths, uint64_t window, uint64_t sinks, void* output,
+                     const float* scale, void* workspace, uint64_t workspace_bytes);
+
 /* -------------------------------------------------------------- Qwen3 model */
 typedef struct dl_qwen3 dl_qwen3;
 
