@@ -39,6 +39,13 @@ __device__ __forceinline__ u32x4 to_bf16(uint32_t codes, float scale) {
 // FP32 values as the exact sum of three BF16 values each (8 significant bits at a
 // time), for products on the BF16 matrix cores that round nothing.  A value that
 // is not finite is its first part alone.
+__device__ __forceinline__ void split(float v, uint32_t (&part)[3]) {  // in the upper halves
+  const bool finite = fabsf(v) < INFINITY;
+  part[0] = v == v ? __float_as_uint(v) & 0xffff0000u : 0x7fc00000u;
+  const float rest = finite ? v - __uint_as_float(part[0]) : 0.0f;
+  part[1] = __float_as_uint(rest) & 0xffff0000u;
+  part[2] = __float_as_uint(rest - __uint_as_float(part[1]));
+}
 struct Parts {
   u32x4 part[3];
 };
@@ -46,19 +53,11 @@ __device__ __forceinline__ Parts split(const float (&x)[8]) {
   Parts p;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    uint32_t high[2], middle[2], low[2];
+    uint32_t lo[3], hi[3];
+    split(x[2 * w], lo);
+    split(x[2 * w + 1], hi);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float v = x[2 * w + e];
-      const bool finite = fabsf(v) < INFINITY;
-      high[e] = v == v ? __float_as_uint(v) & 0xffff0000u : 0x7fc00000u;
-      const float rest = finite ? v - __uint_as_float(high[e]) : 0.0f;
-      middle[e] = __float_as_uint(rest) & 0xffff0000u;
-      low[e] = __float_as_uint(rest - __uint_as_float(middle[e]));
-    }
-    p.part[0][w] = __builtin_amdgcn_perm(high[1], high[0], 0x07060302u);
-    p.part[1][w] = __builtin_amdgcn_perm(middle[1], middle[0], 0x07060302u);
-    p.part[2][w] = __builtin_amdgcn_perm(low[1], low[0], 0x07060302u);
+    for (int i = 0; i < 3; ++i) p.part[i][w] = __builtin_amdgcn_perm(hi[i], lo[i], 0x07060302u);
   }
   return p;
 }

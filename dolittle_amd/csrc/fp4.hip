@@ -98,47 +98,8 @@ struct ProjectArgs {
   const uint8_t *codes, *scales;
   void* y;
   const uint64_t* position;
-  uint32_t rows, in_w, groups, row_tiles;
+  uint32_t rows, in_w, groups;
   uint64_t out_w;
-};
-
-// The product operands of 32 consecutive inputs of a row: four steps of eight.
-template <class T, bool kPieces>
-struct Inputs;
-template <bool kPieces>
-struct Inputs<uint16_t, kPieces> {
-  static constexpr int kParts = 1;
-  u32x4 v[4];
-  __device__ __forceinline__ void load(const uint16_t* row, uint32_t at, uint32_t width) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if constexpr (kPieces) {
-        v[s] = at + 8 * s < width ? *reinterpret_cast<const u32x4*>(row + at + 8 * s) : u32x4{};
-      } else {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t f = at + 8 * s + 2 * w;
-          const uint32_t lo = f < width ? row[f] : 0u, hi = f + 1 < width ? row[f + 1] : 0u;
-          v[s][w] = lo | (hi << 16);
-        }
-      }
-    }
-  }
-  __device__ __forceinline__ void operands(int s, u32x4 (&b)[1]) const { b[0] = v[s]; }
-};
-template <bool kPieces>
-struct Inputs<float, kPieces> {
-  static constexpr int kParts = 3;
-  float v[4][8];
-  __device__ __forceinline__ void load(const float* row, uint32_t at, uint32_t width) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) load_eight<float, kPieces>(row, at + 8 * s, width, v[s]);
-  }
-  __device__ __forceinline__ void operands(int s, u32x4 (&b)[3]) const {
-    const Parts p = split(v[s]);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) b[i] = p.part[i];
-  }
 };
 
 __device__ __forceinline__ f32x4 product(const u32x4& a, const u32x4& b, const f32x4& c) {
@@ -162,104 +123,669 @@ __device__ __forceinline__ void store_four(T* to, const f32x4& v, uint64_t left,
   }
 }
 
-// Up to 16 rows a workgroup, the wavefronts each taking every W-th 256 inputs of
-// 16 kTiles outputs.  A lane's 16 bytes of codes are one group of one output and,
-// converted, the first operand of four products; the same 32 inputs of a row are
-// the second.
-template <class T, bool kPieces, int kTiles, int W>
-__global__ __launch_bounds__(W * 64) void k_project(const ProjectArgs a) {
-  __shared__ f32x4 sums[W][kTiles][64];
-  using In = Inputs<T, kPieces>;
-  constexpr int kParts = In::kParts;
+// Few rows (16 of BF16, 5 of FP32 as three exact parts in columns of their own):
+// bound by the weights' stream.  Eight wavefronts cut the inputs, 256 at a time:
+// wavefront w takes 256 (w + 8 c) .. of every block of 2048 kSlices.  Its rows'
+// inputs stay in registers as second operands; 16 outputs' codes come straight from
+// memory as first operands, a lane's 16 bytes being one group of one output, and
+// are converted in place.  A workgroup walks its tiles of 16 outputs with kAhead - 1
+// slices in flight; a tile's eight sums meet in LDS, where one wavefront adds them up
+// while the others go on.
+constexpr int kProjectWaves = 8;
+
+template <class T>
+constexpr int columns_of = sizeof(T) == 4 ? 5 : 16;  // rows of a workgroup
+
+template <class T, bool kPieces, int kSlices, int kTiles, int kAhead, bool kBlocks>
+__global__ __launch_bounds__(kProjectWaves * 64) __attribute__((amdgpu_waves_per_eu(kSlices == 1 ? 4 : 2)))
+void k_project(const ProjectArgs a, uint32_t per_group) {
+  static_assert(kSlices * kTiles % kAhead == 0, "ring slots are known when compiling");
+  constexpr int W = kProjectWaves, kRows = columns_of<T>;
+  constexpr bool kSplit = sizeof(T) == 4;
+  constexpr int kParts = kSplit ? 3 : 1;
+  __shared__ f32x4 sums[2][W][64];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t i16 = lane % 16, g = lane / 16;
-  const uint32_t row = blockIdx.x % a.row_tiles * 16 + i16;
-  const uint64_t o0 = static_cast<uint64_t>(blockIdx.x / a.row_tiles) * 16 * kTiles;
-  const T* x = static_cast<const T*>(a.x) + static_cast<uint64_t>(min(row, a.rows - 1)) * a.in_w;
-  const uint32_t width = row < a.rows ? a.in_w : 0;  // rows past the last are zeros
-  const u32x4* codes[kTiles];
-  const uint8_t* scales[kTiles];
+  const uint32_t first_row = blockIdx.y * kRows, rows = min(a.rows - first_row, static_cast<uint32_t>(kRows));
+  const T* x = static_cast<const T*>(a.x) + static_cast<uint64_t>(first_row) * a.in_w;
+
+  u32x4 in[kSlices][2][4];  // the inputs of two groups: four product steps each
+  auto load_inputs = [&](uint32_t block) {
+    if constexpr (kSplit || !kPieces) {
+      // The wavefront reads its rows element by element, splits them and takes the
+      // operands from LDS of its own.
+      __shared__ __align__(16) uint16_t parts[W][kParts][kRows][256];
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    const uint64_t o = min(o0 + 16 * t + i16, a.out_w - 1);
-    codes[t] = reinterpret_cast<const u32x4*>(a.codes) + o * a.groups;
-    scales[t] = a.scales + o * a.groups;
-  }
-  f32x4 acc[kTiles];
+      for (int c = 0; c < kSlices; ++c) {
+        const uint32_t base = ((block * kSlices + c) * W + wave) * 256;
+        for (uint32_t r = 0; r < rows; ++r) {
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  u32x4 c[2][kTiles];
-  uint32_t s[2][kTiles];
-  In in[2];
-  // Groups past the last repeat it, with codes of zero under a scale of one.
-  auto load = [&](uint32_t chunk) {
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t at = base + 64 * e + lane;
+            const T v = at < a.in_w ? x[static_cast<uint64_t>(r) * a.in_w + at] : T{};
+            if constexpr (kSplit) {
+              uint32_t part[3];
+              split(v, part);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t group = chunk * 8 + 4 * h + g, at = min(group, a.groups - 1);
+              for (int p = 0; p < 3; ++p) parts[wave][p][r][64 * e + lane] = static_cast<uint16_t>(part[p] >> 16);
+            } else {
+              parts[wave][0][r][64 * e + lane] = v;
+            }
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+        const uint32_t column = min(i16, kParts * rows - 1), part = column / rows, r = column % rows;
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        c[h][t] = load_stream(codes[t] + at);
-        s[h][t] = scales[t][at];
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            in[c][h][s] = *reinterpret_cast<const u32x4*>(&parts[wave][part][r][(4 * h + g) * kGroup + 8 * s]);
+        __builtin_amdgcn_wave_barrier();
       }
-      in[h].load(x, group * kGroup, width);
+    } else {
+#pragma unroll
+      for (int c = 0; c < kSlices; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int s = 0; s < 4; ++s) in[c][h][s] = u32x4{};
+      if (i16 < rows) {  // other columns are not stored
+        const T* row = x + static_cast<uint64_t>(i16) * a.in_w;
+#pragma unroll
+        for (int c = 0; c < kSlices; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t at = (((block * kSlices + c) * W + wave) * 8 + 4 * h + g) * kGroup;
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              in[c][h][s] = at + 8 * s < a.in_w ? *reinterpret_cast<const u32x4*>(row + at + 8 * s) : u32x4{};
+          }
+      }
     }
   };
-  const uint32_t chunks = (a.groups + 7) / 8;
-  uint32_t chunk = wave;
-  if (chunk < chunks) load(chunk);
-  for (; chunk < chunks; chunk += W) {
-    u32x4 now[2][kTiles];
-    float by[2][kTiles];
-    In x_now[2];
+
+  struct Codes {
+    u32x4 code[2];
+    uint32_t scale[2];
+  };
+  Codes ring[kAhead];
+  const uint32_t tiles = static_cast<uint32_t>((a.out_w + 15) / 16), first = blockIdx.x * per_group;
+  const uint32_t count = min(per_group, tiles - first);
+  // Groups past the last repeat it: their inputs are zeros.
+  auto load_codes = [&](Codes& to, uint32_t tile, uint32_t block, int slice) {
+    const uint64_t o = min(static_cast<uint64_t>(first + tile) * 16 + i16, a.out_w - 1) * a.groups;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const bool real = chunk * 8 + 4 * h + g < a.groups;
-      x_now[h] = in[h];
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        now[h][t] = real ? c[h][t] : u32x4{};
-        by[h][t] = scale_of(real ? s[h][t] : 127u);
-      }
+      const uint32_t group = min(((block * kSlices + slice) * W + wave) * 8 + 4 * h + g, a.groups - 1);
+      to.code[h] = load_stream(reinterpret_cast<const u32x4*>(a.codes) + o + group);
+      to.scale[h] = a.scales[o + group];
     }
-    load(min(chunk + W, chunks - 1));
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        u32x4 b[kParts];
-        x_now[h].operands(e, b);
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          const u32x4 w = to_bf16(now[h][t][e], by[h][t]);
-#pragma unroll
-          for (int p = 0; p < kParts; ++p) acc[t] = product(w, b[p], acc[t]);
-        }
-      }
-  }
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t) sums[wave][t][lane] = acc[t];
-  __syncthreads();
-  if (wave >= kTiles) return;
-  f32x4 sum = sums[0][wave][lane];
-#pragma unroll
-  for (int w = 1; w < W; ++w) sum = sum + sums[w][wave][lane];
-  const uint64_t o = o0 + 16 * wave + 4 * g;
-  if (row >= a.rows || o >= a.out_w) return;
+  };
   T* y = static_cast<T*>(a.y) + (a.position ? *a.position * a.out_w : 0);
   const bool whole = a.out_w % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % (4 * sizeof(T)) == 0;
-  store_four(y + row * a.out_w + o, sum, a.out_w - o, whole);
+
+  auto add = [&](const Codes& now, int c, f32x4 sum) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float by = scale_of(now.scale[h]);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) sum = product(to_bf16(now.code[h][s], by), in[c][h][s], sum);
+    }
+    return sum;
+  };
+  // A tile's sums of the eight wavefronts.
+  auto finish = [&](uint32_t tile, const f32x4& acc) {
+    const uint32_t turn = tile % 2;
+    sums[turn][wave][lane] = acc;
+    __syncthreads();
+    if (wave != static_cast<int>(tile % W)) return;
+    f32x4 sum = sums[turn][0][lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) sum = sum + sums[turn][w][lane];
+    if constexpr (kSplit) {  // the low parts' columns into the high ones'
+      f32x4 all = sum;
+#pragma unroll
+      for (int p = 1; p < 3; ++p)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) all[e] = all[e] + __shfl(sum[e], lane + p * static_cast<int>(rows));
+      sum = all;
+    }
+    const uint64_t o = static_cast<uint64_t>(first + tile) * 16 + 4 * g;
+    if (i16 < rows && o < a.out_w) store_four(y + static_cast<uint64_t>(first_row + i16) * a.out_w + o, sum, a.out_w - o, whole);
+  };
+  const f32x4 zeros = {0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (kBlocks) {  // more inputs than the registers hold: read again for every tile
+    const uint32_t blocks = (a.groups + 8 * W * kSlices - 1) / (8 * W * kSlices);
+    for (uint32_t tile = 0; tile < count; ++tile) {
+      f32x4 acc = zeros;
+      for (uint32_t block = 0; block < blocks; ++block) {
+#pragma unroll
+        for (int c = 0; c < kSlices; ++c) load_codes(ring[c], tile, block, c);
+        load_inputs(block);
+#pragma unroll
+        for (int c = 0; c < kSlices; ++c) acc = add(ring[c], c, acc);
+      }
+      finish(tile, acc);
+    }
+  } else {
+    // kTiles tiles from `tile` on, or `count - tile` without more behind them.
+    auto walk = [&](uint32_t tile, auto more) {
+      constexpr bool kMore = decltype(more)::value;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        if (!kMore && tile + t >= count) break;
+        f32x4 acc = zeros;
+#pragma unroll
+        for (int c = 0; c < kSlices; ++c) {
+          const int unit = t * kSlices + c, ahead = unit + kAhead - 1;
+          const uint32_t next = tile + ahead / kSlices;
+          if (kMore || next < count) load_codes(ring[ahead % kAhead], min(next, count - 1), 0, ahead % kSlices);
+          acc = add(ring[unit % kAhead], c, acc);
+        }
+        finish(tile + t, acc);
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < kAhead - 1; ++u)
+      if (u / kSlices < static_cast<int>(count)) load_codes(ring[u], u / kSlices, 0, u % kSlices);
+    load_inputs(0);
+    uint32_t tile = 0;
+    for (; tile + kTiles < count; tile += kTiles) walk(tile, std::true_type{});
+    walk(tile, std::false_type{});
+  }
+}
+
+// The same where rows of scales are whole words: the stream through LDS, so that
+// every load of a wavefront is 1 KiB of one or two rows (16 outputs apart, its lines
+// came at 4 TB/s with the scales and at 5.4 without, this way at 6.7).  A stage is
+// 2048 groups: kRow of 2048 / kRow outputs, M tiles of 16, loaded straight to LDS by
+// all wavefronts, kStages - 1 ahead.  Of its sixteen units of 16 outputs and 256
+// inputs a wavefront takes two.  A barrier a stage says that the stage has landed,
+// that the one before it is read and that its sums are there.  Pieces of a row lie at
+// piece ^ row, so that the 16 rows of an operand lie in distinct banks.
+// A stage's room holds its codes, its scales and the wavefronts' sums.  Objects apart,
+// and none read after loads to it were issued, so that the compiler sees no use of
+// loads in flight and waits for none.
+constexpr int kStageScales = 2048 * kGroupBytes, kStageSums = kStageScales + 2048;
+template <int kStage, int kBytes>
+__device__ __forceinline__ uint8_t* project_stage() {
+  __shared__ __align__(1024) uint8_t room[kBytes];
+  return room;
+}
+
+// s_waitcnt immediate: at most n vector-memory operations and no LDS operation
+// outstanding.
+constexpr unsigned lds_wait(unsigned n) { return vm_wait(n) & ~0x0f00u; }
+// A barrier alone: __syncthreads also waits for all loads to LDS, those of the stages
+// ahead among them.
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <class T, bool kPieces, int kRow, int kBlocks>
+__global__ __launch_bounds__(kProjectWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
+void k_project_staged(const ProjectArgs a, uint32_t per_group) {
+  constexpr int W = kProjectWaves, kRows = columns_of<T>, kOutputs = 2048 / kRow, M = kOutputs / 16;
+  constexpr int kStages = 3, kLoads = 5;  // loads of a wavefront and stage
+  constexpr int kChunks = kRow == 128 ? 2 : 1, kSums = kRow == 128 ? 1 : 2;
+  constexpr int kRoom = kStageSums + kSums * W * 1024;
+  constexpr bool kSplit = sizeof(T) == 4;
+  constexpr int kParts = kSplit ? 3 : 1;
+  static_assert(kBlocks == 1 || kRow == 128, "longer rows are cut into blocks");
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t i16 = lane % 16, g = lane / 16;
+  const uint32_t first_row = blockIdx.y * kRows, rows = min(a.rows - first_row, static_cast<uint32_t>(kRows));
+  const T* x = static_cast<const T*>(a.x) + static_cast<uint64_t>(first_row) * a.in_w;
+  const uint32_t sets = static_cast<uint32_t>((a.out_w + kOutputs - 1) / kOutputs), first = blockIdx.x * per_group;
+  const uint32_t count = min(per_group, sets - first), total = count * kBlocks;
+
+  // The wavefront's chunk of 256 inputs and first tile; its second unit is chunk + 8
+  // of the same tile, or the same chunk of a later tile.
+  const uint32_t chunk = wave % (kRow / 8 < W ? kRow / 8 : W), tile0 = kRow / 8 < W ? wave / (kRow / 8) : 0;
+  constexpr uint32_t kTileStep = kRow == 128 ? 0 : M / 2;
+
+  u32x4 in[kBlocks][kChunks][2][4];
+  if constexpr (kSplit || !kPieces) {
+    // Element by element through LDS of the wavefront's own, in the stage loaded last.
+    constexpr int kHalf = 128;
+    uint16_t* parts = reinterpret_cast<uint16_t*>(project_stage<kStages - 1, kRoom>()) + wave * (kParts * kRows * kHalf);
+    static_assert(W * kParts * kRows * kHalf * 2 <= kRoom, "parts outgrow a stage");
+    T v[2][2][kRows][2];  // a chunk's elements, loaded a chunk ahead; rows past the last repeat it
+    auto load = [&](T (&to)[2][kRows][2], int batch) __attribute__((always_inline)) {
+      const uint32_t base = batch / kChunks * kRow * kGroup + (chunk + 8 * (batch % kChunks)) * 256 + lane;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            to[h][r][e] = x[static_cast<uint64_t>(min(static_cast<uint32_t>(r), rows - 1)) * a.in_w + min(base + h * kHalf + 64 * e, a.in_w - 1)];
+    };
+    const uint32_t column = min(i16, kParts * rows - 1), part = column / rows, in_part = column % rows;
+    load(v[0], 0);
+#pragma unroll
+    for (int batch = 0; batch < kBlocks * kChunks; ++batch) {
+      const int b = batch / kChunks, c = batch % kChunks;
+      if (batch + 1 < kBlocks * kChunks) load(v[(batch + 1) % 2], batch + 1);
+      const uint32_t base = b * kRow * kGroup + (chunk + 8 * c) * 256 + lane;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const T in_row = base + h * kHalf + 64 * e < a.in_w ? v[batch % 2][h][r][e] : T{};
+            uint16_t* to = parts + r * kHalf + 64 * e + lane;
+            if constexpr (kSplit) {
+              uint32_t three[3];
+              split(in_row, three);
+#pragma unroll
+              for (int p = 0; p < 3; ++p) to[p * kRows * kHalf] = static_cast<uint16_t>(three[p] >> 16);
+            } else {
+              *to = in_row;
+            }
+          }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          in[b][c][h][s] = *reinterpret_cast<const u32x4*>(parts + (part * kRows + in_part) * kHalf + g * kGroup + 8 * s);
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int s = 0; s < 4; ++s) in[b][c][h][s] = u32x4{};
+    if (i16 < rows) {  // other columns are not stored
+      const T* row = x + static_cast<uint64_t>(i16) * a.in_w;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t at = b * kRow * kGroup + (chunk + 8 * c) * 256 + (4 * h + g) * kGroup;
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              in[b][c][h][s] = at + 8 * s < a.in_w ? *reinterpret_cast<const u32x4*>(row + at + 8 * s) : u32x4{};
+          }
+    }
+  }
+
+  // Groups past the last repeat it, their inputs are zeros; outputs past the last
+  // repeat it and are not stored.
+  auto code_place = [&](int i, uint32_t block, uint32_t left) {
+    const uint32_t at = (i * W + wave) * 64, in_row = at % kRow + lane;  // kRow 128, 64: one row for the wavefront
+    const uint32_t row = at / kRow + (kRow < 64 ? in_row / kRow : 0), piece = in_row % kRow ^ row % 16;
+    return (min(row, left) * a.groups + min(block * kRow + piece, a.groups - 1)) * kGroupBytes;
+  };
+  constexpr uint32_t kWords = kRow / 4, kWordSwizzle = kWords < 16 ? kWords : 16;  // words of four scales
+  auto scale_place = [&](uint32_t block, uint32_t left) {
+    const uint32_t slot = wave * 64 + lane, row = slot / kWords;
+    return (min(row, left) * (a.groups / 4) + min(block * kWords + (slot % kWords ^ row % kWordSwizzle), a.groups / 4 - 1)) * 4;
+  };
+  auto issue = [&](uint8_t* room, uint32_t stage) __attribute__((always_inline)) {
+    const uint32_t block = kBlocks == 1 ? 0 : stage % kBlocks;
+    const uint64_t o0 = static_cast<uint64_t>(first + stage / kBlocks) * kOutputs;
+    const uint8_t* codes = a.codes + o0 * a.groups * kGroupBytes;
+    const uint8_t* scales = a.scales + o0 * a.groups;
+    const uint32_t left = a.out_w - o0 < kOutputs ? static_cast<uint32_t>(a.out_w - o0) - 1 : kOutputs - 1;
+    uint32_t at[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads - 1; ++i) at[i] = code_place(i, block, left);
+    at[kLoads - 1] = scale_place(block, left);
+#pragma unroll
+    for (int i = 0; i < kLoads - 1; ++i)
+      __builtin_amdgcn_global_load_lds((const global_ptr*)(codes + at[i]), (lds_ptr*)(room + (i * W + wave) * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((const global_ptr*)(scales + at[kLoads - 1]),
+                                     (lds_ptr*)(room + kStageScales + wave * 256), 4, 0, 0);
+  };
+  f32x4 acc[kSums];
+  auto step = [&](const uint8_t* room, auto constant) __attribute__((always_inline)) {
+    constexpr int block = decltype(constant)::value;
+    if (block == 0)
+#pragma unroll
+      for (f32x4& v : acc) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int c = kRow == 128 ? u : 0, to = kRow == 128 ? 0 : u;
+      const uint32_t row = (tile0 + u * kTileStep) * 16 + i16;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t piece = (chunk + 8 * c) * 8 + 4 * h + g, word = piece / 4;
+        const u32x4 code = *reinterpret_cast<const u32x4*>(room + (row * kRow + (piece ^ i16)) * kGroupBytes);
+        const uint32_t scale =
+            *reinterpret_cast<const uint32_t*>(room + kStageScales + (row * kWords + (word ^ row % kWordSwizzle)) * 4);
+        const float by = scale_of(scale >> (8 * g) & 255u);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) acc[to] = product(to_bf16(code[s], by), in[block][c][h][s], acc[to]);
+      }
+    }
+  };
+  T* y = static_cast<T*>(a.y) + (a.position ? *a.position * a.out_w : 0);
+  const bool whole = a.out_w % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % (4 * sizeof(T)) == 0;
+  // The sums of set n, whose last stage has this room, by one wavefront a tile.
+  auto finish = [&](const uint8_t* room, uint32_t n) __attribute__((always_inline)) {
+    const f32x4* sums = reinterpret_cast<const f32x4*>(room + kStageSums) + lane;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      if (wave != static_cast<int>((n * M + m) % W)) continue;
+      constexpr int kOf = kRow / 8 < W ? kRow / 8 : W;  // wavefronts that have a part of a tile
+      const int from = kRow / 8 < W ? m % (W / kOf) * kOf : 0, which = kRow == 128 ? 0 : m / (M / 2);
+      f32x4 sum = sums[(which * W + from) * 64];
+#pragma unroll
+      for (int w = 1; w < kOf; ++w) sum = sum + sums[(which * W + from + w) * 64];
+      if constexpr (kSplit) {  // the low parts' columns into the high ones'
+        f32x4 all = sum;
+#pragma unroll
+        for (int p = 1; p < 3; ++p)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) all[e] = all[e] + __shfl(sum[e], lane + p * static_cast<int>(rows));
+        sum = all;
+      }
+      const uint64_t o = (static_cast<uint64_t>(first + n) * M + m) * 16 + 4 * g;
+      if (i16 < rows && o < a.out_w) store_four(y + static_cast<uint64_t>(first_row + i16) * a.out_w + o, sum, a.out_w - o, whole);
+    }
+  };
+  auto work = [&](uint8_t* room, uint32_t block) __attribute__((always_inline)) {
+    if (block == 0) step(room, std::integral_constant<int, 0>{});
+    if constexpr (kBlocks > 1)
+      if (block == 1) step(room, std::integral_constant<int, 1>{});
+    if constexpr (kBlocks > 2)
+      if (block == 2) step(room, std::integral_constant<int, 2>{});
+    if (block == kBlocks - 1)
+#pragma unroll
+      for (int u = 0; u < kSums; ++u) reinterpret_cast<f32x4*>(room + kStageSums)[(u * W + wave) * 64 + lane] = acc[u];
+  };
+  auto finish_before = [&](const uint8_t* room, uint32_t stage) __attribute__((always_inline)) {
+    if (stage && stage % kBlocks == 0) finish(room, stage / kBlocks - 1);
+  };
+  // A stage with two more behind it: it has landed when only the next one's loads are
+  // under way.  No load here lies under a condition: the compiler would wait for all of
+  // them before every read.
+  auto turn = [&](auto slot, uint32_t stage) __attribute__((always_inline)) {
+    constexpr int kSlot = decltype(slot)::value, kBefore = (kSlot + kStages - 1) % kStages;
+    __builtin_amdgcn_s_waitcnt(lds_wait((kStages - 2) * kLoads));
+    meet();
+    finish_before(project_stage<kBefore, kRoom>(), stage);
+    issue(project_stage<kBefore, kRoom>(), stage + kStages - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    work(project_stage<kSlot, kRoom>(), kBlocks == kStages ? kSlot : stage % kBlocks);
+  };
+  auto room_of = [&](uint32_t stage) {
+    const uint32_t slot = stage % kStages;
+    return slot == 0 ? project_stage<0, kRoom>() : slot == 1 ? project_stage<1, kRoom>() : project_stage<2, kRoom>();
+  };
+  uint32_t stage = 0;
+  if (total < kStages) {
+    issue(project_stage<0, kRoom>(), 0);
+    if (total > 1) issue(project_stage<1, kRoom>(), 1);
+  } else {
+    issue(project_stage<0, kRoom>(), 0);
+    issue(project_stage<1, kRoom>(), 1);
+    __builtin_amdgcn_s_waitcnt(vm_wait(2 * kLoads));  // the inputs
+    for (;;) {
+      turn(std::integral_constant<int, 0>{}, stage++);
+      if (stage + kStages - 1 >= total) break;
+      turn(std::integral_constant<int, 1>{}, stage++);
+      if (stage + kStages - 1 >= total) break;
+      turn(std::integral_constant<int, 2>{}, stage++);
+      if (stage + kStages - 1 >= total) break;
+    }
+  }
+  for (; stage < total; ++stage) {  // the last stages, which have no loads behind them
+    __builtin_amdgcn_s_waitcnt(lds_wait(0));
+    meet();
+    finish_before(room_of(stage + kStages - 1), stage);
+    work(room_of(stage), stage % kBlocks);
+  }
+  __syncthreads();
+  finish(room_of(total - 1), count - 1);
+}
+
+// What loads to LDS take for inputs past the width.
+__device__ const u32x4 zero_piece = {0, 0, 0, 0};
+
+// Many rows: four wavefronts share 32 kRowTiles rows, 128 inputs at a time through
+// LDS, loaded kStages - 1 steps ahead; each has 32 outputs of its own, whose codes come
+// straight from memory as far ahead, so that every code is converted once for all the
+// rows.  32 x 32 products: 2440 TFLOP/s against 1460 of 16 x 16 ones.
+template <int kStage, int kBytes>
+__device__ __forceinline__ uint8_t* many_stage() {
+  __shared__ __align__(1024) uint8_t room[kBytes];
+  return room;
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kManyOutputs = 128;
+
+template <class T, bool kPieces, bool kWords, int kRowTiles>
+__global__ __launch_bounds__(256) void k_project_many(const ProjectArgs a, uint32_t row_tiles) {
+  constexpr int W = 4, kRows = 32 * kRowTiles, kParts = sizeof(T) == 4 ? 3 : 1, kRowBytes = 256;
+  // A ring of steps where rows go to LDS directly, else two, rows through registers.
+  constexpr int kStages = kPieces && sizeof(T) == 2 ? 4 : 2;
+  constexpr int kPart = kRows * kRowBytes, kPer = kRows * 16 / 256;  // 16-byte pieces of a thread
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t i32 = lane % 32, half = lane / 32;
+  // XCD x takes the output tiles x, x + 8, ..., and all row tiles of one, which read
+  // the same codes.
+  const uint32_t in_xcd = blockIdx.x / 8, out_tile = in_xcd / row_tiles * 8 + blockIdx.x % 8, row0 = in_xcd % row_tiles * kRows;
+  const uint64_t o0 = static_cast<uint64_t>(out_tile) * kManyOutputs + 32 * wave;
+  if (static_cast<uint64_t>(out_tile) * kManyOutputs >= a.out_w) return;
+  const T* x = static_cast<const T*>(a.x);
+  const uint32_t steps = (a.groups + 3) / 4;
+
+  const uint64_t output = min(o0 + i32, a.out_w - 1) * a.groups;
+  const u32x4* codes = reinterpret_cast<const u32x4*>(a.codes) + output;
+  const uint8_t* scales = a.scales + output;
+  // Two of a step's four groups: 2 h + half.
+  struct Codes {
+    u32x4 code[2];
+    uint32_t scale[kWords ? 1 : 2];
+  };
+  Codes ring[kStages];
+  auto load_codes = [&](Codes& to, uint32_t step) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // groups past the last repeat it: their inputs are zeros
+      const uint32_t group = min(step * 4 + 2 * h + half, a.groups - 1);
+      to.code[h] = codes[group];
+      if constexpr (!kWords) to.scale[h] = scales[group];
+    }
+    if constexpr (kWords) to.scale[0] = *reinterpret_cast<const uint32_t*>(scales + min(step * 4, a.groups - 4));
+  };
+  auto factor = [&](const Codes& from, int h) __attribute__((always_inline)) {
+    if constexpr (kWords) return scale_of(from.scale[0] >> (16 * h + 8 * half) & 255u);
+    else return scale_of(from.scale[h]);
+  };
+  // Piece p (eight inputs) of row r lies at p ^ r.
+  constexpr bool kDirect = kPieces && sizeof(T) == 2;
+  float held[kDirect ? 1 : kPer][8];
+  auto load_rows = [&](uint8_t* room, uint32_t step) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t slot = i * 256 + threadIdx.x, r = slot / 16, piece = slot % 16 ^ r % 16, at = step * 128 + piece * 8;
+      const T* row = x + static_cast<uint64_t>(min(row0 + r, a.rows - 1)) * a.in_w;
+      if constexpr (kDirect) {
+        const void* from = at < a.in_w ? static_cast<const void*>(row + at) : &zero_piece;
+        __builtin_amdgcn_global_load_lds((const global_ptr*)from, (lds_ptr*)(room + (i * W + wave) * 1024), 16, 0, 0);
+      } else {
+        load_eight<T, kPieces>(row, at, a.in_w, held[i]);
+      }
+    }
+  };
+  auto store_rows = [&](uint8_t* room) __attribute__((always_inline)) {
+    if constexpr (!kDirect) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        uint8_t* to = room + (i * 256 + threadIdx.x) * 16;
+        if constexpr (kParts == 3) {
+          const Parts p = split(held[i]);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x4*>(to + k * kPart) = p.part[k];
+        } else {
+          u32x4 v;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) v[w] = __float_as_uint(held[i][2 * w]) >> 16 | (__float_as_uint(held[i][2 * w + 1]) & 0xffff0000u);
+          *reinterpret_cast<u32x4*>(to) = v;
+        }
+      }
+    }
+  };
+  f32x16 acc[kRowTiles];
+#pragma unroll
+  for (int r = 0; r < kRowTiles; ++r) acc[r] = f32x16{};
+  // Rows of a product step (16 inputs) are read two steps before they are multiplied,
+  // and codes converted one step before.
+  constexpr int kProducts = kRowTiles * kParts;
+  u32x4 v[3][kProducts], weight[2];
+  auto read = [&](const uint8_t* room, int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < kRowTiles; ++r)
+#pragma unroll
+      for (int p = 0; p < kParts; ++p)
+        v[s % 3][r * kParts + p] = *reinterpret_cast<const u32x4*>(
+            room + p * kPart + (32 * r + i32) * kRowBytes + ((8 * (s / 4) + 4 * half + s % 4) ^ i32 % 16) * 16);
+  };
+  auto convert = [&](const Codes& from, int s) __attribute__((always_inline)) {
+    weight[s % 2] = to_bf16(from.code[s / 4][s % 4], factor(from, s / 4));
+  };
+  auto compute = [&](const uint8_t* room, const Codes& from) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      if (s < 6) read(room, s + 2);
+      if (s < 7) convert(from, s + 1);
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i)
+        acc[i / kParts] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, weight[s % 2]),
+                                                                  __builtin_bit_cast(bf16x8, v[s % 3][i]), acc[i / kParts], 0, 0, 0);
+      if (s < 7) {
+        if (s < 6) __builtin_amdgcn_sched_group_barrier(0x100, kProducts, 0);
+#pragma unroll
+        for (int i = 0; i < kProducts; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x2, (6 + kProducts - 1) / kProducts, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  constexpr int kBytes = kParts * kPart, kAhead = kStages - 1;
+  // Steps past the last have zeros for rows.  No load lies under a condition, and the
+  // loop is left at its end alone: the compiler would wait for all loads in flight.
+  auto turn = [&](auto slot, uint32_t step) __attribute__((always_inline)) {
+    constexpr int kSlot = decltype(slot)::value, kNext = (kSlot + kAhead) % kStages;
+    __builtin_amdgcn_s_waitcnt(lds_wait(kDirect ? (kAhead - 1) * (kPer + (kWords ? 3 : 4)) : 63));  // this step's rows
+    meet();
+    read(many_stage<kSlot, kBytes>(), 0);
+    read(many_stage<kSlot, kBytes>(), 1);
+    __builtin_amdgcn_sched_barrier(0);
+    load_rows(many_stage<kNext, kBytes>(), step + kAhead);
+    load_codes(ring[kNext], step + kAhead);
+    convert(ring[kSlot], 0);
+    __builtin_amdgcn_sched_barrier(0);
+    compute(many_stage<kSlot, kBytes>(), ring[kSlot]);
+    store_rows(many_stage<kNext, kBytes>());
+  };
+  auto first = [&](auto slot) __attribute__((always_inline)) {
+    constexpr int kSlot = decltype(slot)::value;
+    load_rows(many_stage<kSlot, kBytes>(), kSlot);
+    load_codes(ring[kSlot], kSlot);
+    store_rows(many_stage<kSlot, kBytes>());
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  first(std::integral_constant<int, 0>{});
+  if constexpr (kAhead > 1) first(std::integral_constant<int, 1>{});
+  if constexpr (kAhead > 2) first(std::integral_constant<int, 2>{});
+  for (uint32_t step = 0; step < steps; step += kStages) {
+    turn(std::integral_constant<int, 0>{}, step);
+    turn(std::integral_constant<int, 1>{}, step + 1);
+    if constexpr (kStages > 2) turn(std::integral_constant<int, 2>{}, step + 2);
+    if constexpr (kStages > 3) turn(std::integral_constant<int, 3>{}, step + 3);
+  }
+  T* y = static_cast<T*>(a.y) + (a.position ? *a.position * a.out_w : 0);
+  const bool whole = a.out_w % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % (4 * sizeof(T)) == 0;
+#pragma unroll
+  for (int r = 0; r < kRowTiles; ++r) {
+    const uint32_t row = row0 + 32 * r + i32;
+    if (row >= a.rows) continue;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint64_t o = o0 + 8 * q + 4 * half;
+      const f32x4 four = {acc[r][4 * q], acc[r][4 * q + 1], acc[r][4 * q + 2], acc[r][4 * q + 3]};
+      if (o < a.out_w) store_four(y + static_cast<uint64_t>(row) * a.out_w + o, four, a.out_w - o, whole);
+    }
+  }
 }
 
 template <class T, bool kPieces>
-void launch_project(hipStream_t s, ProjectArgs& a) {
-  auto run = [&](auto tiles) {
-    constexpr int kTiles = decltype(tiles)::value, kWaves = 8;
-    const uint64_t blocks = ceil_div(a.out_w, 16 * kTiles) * a.row_tiles;
-    require(blocks <= (1u << 23), "too many workgroups", DL_LENGTH_ERROR);
-    k_project<T, kPieces, kTiles, kWaves><<<static_cast<unsigned>(blocks), kWaves * 64, 0, s>>>(a);
+void launch_project(hipStream_t s, const ProjectArgs& a) {
+  const bool words = a.groups % 4 == 0 && reinterpret_cast<uintptr_t>(a.scales) % 4 == 0;
+  // Few rows read the weights once per 16 (FP32 5); many convert them once per 32 or 64
+  // and need tiles for most compute units.  4096 x 4096, rows 24, 48 and 128: few 11, 18
+  // and 45 us, many by 32 rows 17, 17 and 18, by 64 19, 20 and 20; 4096 x 24576, 48 and
+  // 128 rows: few 40 and 97, by 32 42 and 61, by 64 29 and 51.
+  if (a.rows > (sizeof(T) == 4 ? 20 : 32)) {
+    auto many = [&](auto whole_words, auto tiles) {
+      constexpr int kRowTiles = decltype(tiles)::value;
+      const uint64_t row_tiles = ceil_div(a.rows, 32 * kRowTiles), out_tiles = ceil_div(ceil_div(a.out_w, kManyOutputs), 8) * 8;
+      require(row_tiles * out_tiles <= (1u << 23), "too many workgroups", DL_LENGTH_ERROR);
+      k_project_many<T, kPieces, decltype(whole_words)::value, kRowTiles>
+          <<<static_cast<unsigned>(row_tiles * out_tiles), 256, 0, s>>>(a, static_cast<uint32_t>(row_tiles));
+    };
+    auto by_rows = [&](auto whole_words) {
+      if constexpr (sizeof(T) == 2) {
+        if (ceil_div(a.rows, 64) * ceil_div(a.out_w, kManyOutputs) > 128) return many(whole_words, std::integral_constant<int, 2>{});
+      }
+      many(whole_words, std::integral_constant<int, 1>{});
+    };
+    words ? by_rows(std::true_type{}) : by_rows(std::false_type{});
+    return;
+  }
+  const uint64_t row_tiles = ceil_div(a.rows, columns_of<T>);
+  require(row_tiles <= 65535, "too many rows", DL_LENGTH_ERROR);
+#define I(n) std::integral_constant<int, n>{}
+  if (words && a.groups <= 384) {
+    auto run = [&](auto row, auto blocks) {
+      constexpr int kRow = decltype(row)::value, kBlocks = decltype(blocks)::value;
+      const uint64_t sets = ceil_div(a.out_w, 2048 / kRow), per_group = ceil_div(sets, 256);
+      const dim3 grid(static_cast<unsigned>(ceil_div(sets, per_group)), static_cast<unsigned>(row_tiles));
+      k_project_staged<T, kPieces, kRow, kBlocks><<<grid, kProjectWaves * 64, 0, s>>>(a, static_cast<uint32_t>(per_group));
+    };
+    if (a.groups <= 32)
+      run(I(32), I(1));
+    else if (a.groups <= 64)
+      run(I(64), I(1));
+    else if (a.groups <= 128)
+      run(I(128), I(1));
+    else if (a.groups <= 256)
+      run(I(128), I(2));
+    else
+      run(I(128), I(3));
+    return;
+  }
+  const uint64_t tiles = ceil_div(a.out_w, 16), slices = ceil_div(ceil_div(a.groups, 8), kProjectWaves);
+  auto run = [&](auto n, auto count, auto ahead, auto many) {
+    constexpr int kSlices = decltype(n)::value, kTiles = decltype(count)::value, kAhead = decltype(ahead)::value;
+    const uint64_t per_group = ceil_div(tiles, kSlices == 1 ? 512 : 256);
+    const dim3 grid(static_cast<unsigned>(ceil_div(tiles, per_group)), static_cast<unsigned>(row_tiles));
+    k_project<T, kPieces, kSlices, kTiles, kAhead, decltype(many)::value>
+        <<<grid, kProjectWaves * 64, 0, s>>>(a, static_cast<uint32_t>(per_group));
   };
-  a.row_tiles = static_cast<uint32_t>(ceil_div(a.rows, 16));
-  run(std::integral_constant<int, 1>{});
+  if (slices == 1)
+    run(I(1), I(4), I(4), std::false_type{});
+  else if (slices == 2)
+    run(I(2), I(4), I(8), std::false_type{});
+  else
+    run(I(2), I(1), I(2), std::true_type{});
+#undef I
 }
 
 // --------------------------------------------------------------------- append
@@ -448,7 +974,7 @@ int dl_projection_fp4(dl_queue* queue, int dtype, const void* input, const void*
     dl::enter(queue);
     ProjectArgs a{input, static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), output, output_position,
                   static_cast<uint32_t>(rows), static_cast<uint32_t>(input_width),
-                  static_cast<uint32_t>(groups_of(input_width)), 0, output_width};
+                  static_cast<uint32_t>(groups_of(input_width)), output_width};
     with_type(dtype, whole_rows(dtype, input_width, input), [&](auto type, auto pieces) {
       launch_project<decltype(type), decltype(pieces)::value>(queue->stream, a);
     });

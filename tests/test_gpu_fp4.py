@@ -133,7 +133,8 @@ def project(device, queue, dtype, x, codes, scales, rows, inputs, outputs, shift
 
 
 PROJECTIONS = [(1, 32, 16), (1, 4096, 1024), (2, 1000, 777), (3, 12288, 33), (5, 31, 1), (8, 256, 4096), (16, 288, 50), (17, 4096, 64),
-               (33, 160, 100), (64, 512, 129), (100, 2048, 300), (257, 96, 260), (130, 33, 65)]
+               (33, 160, 100), (64, 512, 129), (100, 2048, 300), (257, 96, 260), (130, 33, 65),
+               (2, 8100, 40), (4, 6145, 20), (3, 12500, 37), (1, 30000, 16), (6, 1999, 2100), (1, 64, 9000)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
