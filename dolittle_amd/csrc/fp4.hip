@@ -124,180 +124,17 @@ __device__ __forceinline__ void store_four(T* to, const f32x4& v, uint64_t left,
 }
 
 // Few rows (16 of BF16, 5 of FP32 as three exact parts in columns of their own):
-// bound by the weights' stream.  Eight wavefronts cut the inputs, 256 at a time:
-// wavefront w takes 256 (w + 8 c) .. of every block of 2048 kSlices.  Its rows'
-// inputs stay in registers as second operands; 16 outputs' codes come straight from
-// memory as first operands, a lane's 16 bytes being one group of one output, and
-// are converted in place.  A workgroup walks its tiles of 16 outputs with kAhead - 1
-// slices in flight; a tile's eight sums meet in LDS, where one wavefront adds them up
-// while the others go on.
+// bound by the weights' stream.  Eight wavefronts cut the inputs, 256 at a time.
+// Inputs are the products' second operands; 16 outputs' codes are first operands, a
+// lane's 16 bytes being one group of one output, converted in place.
 constexpr int kProjectWaves = 8;
 
 template <class T>
 constexpr int columns_of = sizeof(T) == 4 ? 5 : 16;  // rows of a workgroup
 
-template <class T, bool kPieces, int kSlices, int kTiles, int kAhead, bool kBlocks>
-__global__ __launch_bounds__(kProjectWaves * 64) __attribute__((amdgpu_waves_per_eu(kSlices == 1 ? 4 : 2)))
-void k_project(const ProjectArgs a, uint32_t per_group) {
-  static_assert(kSlices * kTiles % kAhead == 0, "ring slots are known when compiling");
-  constexpr int W = kProjectWaves, kRows = columns_of<T>;
-  constexpr bool kSplit = sizeof(T) == 4;
-  constexpr int kParts = kSplit ? 3 : 1;
-  __shared__ f32x4 sums[2][W][64];
-  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const uint32_t i16 = lane % 16, g = lane / 16;
-  const uint32_t first_row = blockIdx.y * kRows, rows = min(a.rows - first_row, static_cast<uint32_t>(kRows));
-  const T* x = static_cast<const T*>(a.x) + static_cast<uint64_t>(first_row) * a.in_w;
-
-  u32x4 in[kSlices][2][4];  // the inputs of two groups: four product steps each
-  auto load_inputs = [&](uint32_t block) {
-    if constexpr (kSplit || !kPieces) {
-      // The wavefront reads its rows element by element, splits them and takes the
-      // operands from LDS of its own.
-      __shared__ __align__(16) uint16_t parts[W][kParts][kRows][256];
-#pragma unroll
-      for (int c = 0; c < kSlices; ++c) {
-        const uint32_t base = ((block * kSlices + c) * W + wave) * 256;
-        for (uint32_t r = 0; r < rows; ++r) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t at = base + 64 * e + lane;
-            const T v = at < a.in_w ? x[static_cast<uint64_t>(r) * a.in_w + at] : T{};
-            if constexpr (kSplit) {
-              uint32_t part[3];
-              split(v, part);
-#pragma unroll
-              for (int p = 0; p < 3; ++p) parts[wave][p][r][64 * e + lane] = static_cast<uint16_t>(part[p] >> 16);
-            } else {
-              parts[wave][0][r][64 * e + lane] = v;
-            }
-          }
-        }
-        __builtin_amdgcn_wave_barrier();
-        const uint32_t column = min(i16, kParts * rows - 1), part = column / rows, r = column % rows;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int s = 0; s < 4; ++s)
-            in[c][h][s] = *reinterpret_cast<const u32x4*>(&parts[wave][part][r][(4 * h + g) * kGroup + 8 * s]);
-        __builtin_amdgcn_wave_barrier();
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < kSlices; ++c)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int s = 0; s < 4; ++s) in[c][h][s] = u32x4{};
-      if (i16 < rows) {  // other columns are not stored
-        const T* row = x + static_cast<uint64_t>(i16) * a.in_w;
-#pragma unroll
-        for (int c = 0; c < kSlices; ++c)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t at = (((block * kSlices + c) * W + wave) * 8 + 4 * h + g) * kGroup;
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-              in[c][h][s] = at + 8 * s < a.in_w ? *reinterpret_cast<const u32x4*>(row + at + 8 * s) : u32x4{};
-          }
-      }
-    }
-  };
-
-  struct Codes {
-    u32x4 code[2];
-    uint32_t scale[2];
-  };
-  Codes ring[kAhead];
-  const uint32_t tiles = static_cast<uint32_t>((a.out_w + 15) / 16), first = blockIdx.x * per_group;
-  const uint32_t count = min(per_group, tiles - first);
-  // Groups past the last repeat it: their inputs are zeros.
-  auto load_codes = [&](Codes& to, uint32_t tile, uint32_t block, int slice) {
-    const uint64_t o = min(static_cast<uint64_t>(first + tile) * 16 + i16, a.out_w - 1) * a.groups;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t group = min(((block * kSlices + slice) * W + wave) * 8 + 4 * h + g, a.groups - 1);
-      to.code[h] = load_stream(reinterpret_cast<const u32x4*>(a.codes) + o + group);
-      to.scale[h] = a.scales[o + group];
-    }
-  };
-  T* y = static_cast<T*>(a.y) + (a.position ? *a.position * a.out_w : 0);
-  const bool whole = a.out_w % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % (4 * sizeof(T)) == 0;
-
-  auto add = [&](const Codes& now, int c, f32x4 sum) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float by = scale_of(now.scale[h]);
-#pragma unroll
-      for (int s = 0; s < 4; ++s) sum = product(to_bf16(now.code[h][s], by), in[c][h][s], sum);
-    }
-    return sum;
-  };
-  // A tile's sums of the eight wavefronts.
-  auto finish = [&](uint32_t tile, const f32x4& acc) {
-    const uint32_t turn = tile % 2;
-    sums[turn][wave][lane] = acc;
-    __syncthreads();
-    if (wave != static_cast<int>(tile % W)) return;
-    f32x4 sum = sums[turn][0][lane];
-#pragma unroll
-    for (int w = 1; w < W; ++w) sum = sum + sums[turn][w][lane];
-    if constexpr (kSplit) {  // the low parts' columns into the high ones'
-      f32x4 all = sum;
-#pragma unroll
-      for (int p = 1; p < 3; ++p)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) all[e] = all[e] + __shfl(sum[e], lane + p * static_cast<int>(rows));
-      sum = all;
-    }
-    const uint64_t o = static_cast<uint64_t>(first + tile) * 16 + 4 * g;
-    if (i16 < rows && o < a.out_w) store_four(y + static_cast<uint64_t>(first_row + i16) * a.out_w + o, sum, a.out_w - o, whole);
-  };
-  const f32x4 zeros = {0.0f, 0.0f, 0.0f, 0.0f};
-  if constexpr (kBlocks) {  // more inputs than the registers hold: read again for every tile
-    const uint32_t blocks = (a.groups + 8 * W * kSlices - 1) / (8 * W * kSlices);
-    for (uint32_t tile = 0; tile < count; ++tile) {
-      f32x4 acc = zeros;
-      for (uint32_t block = 0; block < blocks; ++block) {
-#pragma unroll
-        for (int c = 0; c < kSlices; ++c) load_codes(ring[c], tile, block, c);
-        load_inputs(block);
-#pragma unroll
-        for (int c = 0; c < kSlices; ++c) acc = add(ring[c], c, acc);
-      }
-      finish(tile, acc);
-    }
-  } else {
-    // kTiles tiles from `tile` on, or `count - tile` without more behind them.
-    auto walk = [&](uint32_t tile, auto more) {
-      constexpr bool kMore = decltype(more)::value;
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        if (!kMore && tile + t >= count) break;
-        f32x4 acc = zeros;
-#pragma unroll
-        for (int c = 0; c < kSlices; ++c) {
-          const int unit = t * kSlices + c, ahead = unit + kAhead - 1;
-          const uint32_t next = tile + ahead / kSlices;
-          if (kMore || next < count) load_codes(ring[ahead % kAhead], min(next, count - 1), 0, ahead % kSlices);
-          acc = add(ring[unit % kAhead], c, acc);
-        }
-        finish(tile + t, acc);
-      }
-    };
-#pragma unroll
-    for (int u = 0; u < kAhead - 1; ++u)
-      if (u / kSlices < static_cast<int>(count)) load_codes(ring[u], u / kSlices, 0, u % kSlices);
-    load_inputs(0);
-    uint32_t tile = 0;
-    for (; tile + kTiles < count; tile += kTiles) walk(tile, std::true_type{});
-    walk(tile, std::false_type{});
-  }
-}
-
-// The same where rows of scales are whole words: the stream through LDS, so that
-// every load of a wavefront is 1 KiB of one or two rows (16 outputs apart, its lines
-// came at 4 TB/s with the scales and at 5.4 without, this way at 6.7).  A stage is
+// The stream goes through LDS, so that every load of a wavefront is 1 KiB of one or two
+// rows: read as operands, 16 rows at a time, it came at 4 TB/s with the scales and at
+// 5.4 without, this way at 6.7.  A stage is
 // 2048 groups: kRow of 2048 / kRow outputs, M tiles of 16, loaded straight to LDS by
 // all wavefronts, kStages - 1 ahead.  Of its sixteen units of 16 outputs and 256
 // inputs a wavefront takes two.  A barrier a stage says that the stage has landed,
@@ -324,11 +161,11 @@ __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
 }
 
-template <class T, bool kPieces, int kRow, int kBlocks>
+template <class T, bool kPieces, bool kWhole, int kRow, int kBlocks>
 __global__ __launch_bounds__(kProjectWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
 void k_project_staged(const ProjectArgs a, uint32_t per_group) {
   constexpr int W = kProjectWaves, kRows = columns_of<T>, kOutputs = 2048 / kRow, M = kOutputs / 16;
-  constexpr int kStages = 3, kLoads = 5;  // loads of a wavefront and stage
+  constexpr int kStages = 3, kLoads = kWhole ? 5 : 8;  // loads of a wavefront and stage
   constexpr int kChunks = kRow == 128 ? 2 : 1, kSums = kRow == 128 ? 1 : 2;
   constexpr int kRoom = kStageSums + kSums * W * 1024;
   constexpr bool kSplit = sizeof(T) == 4;
@@ -431,24 +268,37 @@ void k_project_staged(const ProjectArgs a, uint32_t per_group) {
     const uint32_t slot = wave * 64 + lane, row = slot / kWords;
     return (min(row, left) * (a.groups / 4) + min(block * kWords + (slot % kWords ^ row % kWordSwizzle), a.groups / 4 - 1)) * 4;
   };
-  auto issue = [&](uint8_t* room, uint32_t stage) __attribute__((always_inline)) {
+  // Scales of the wavefront's two units, where their rows are not whole words.
+  struct Held {
+    uint32_t scale[2][2];
+  };
+  Held ring[kStages];
+  auto issue = [&](uint8_t* room, Held& held, uint32_t stage) __attribute__((always_inline)) {
     const uint32_t block = kBlocks == 1 ? 0 : stage % kBlocks;
     const uint64_t o0 = static_cast<uint64_t>(first + stage / kBlocks) * kOutputs;
     const uint8_t* codes = a.codes + o0 * a.groups * kGroupBytes;
     const uint8_t* scales = a.scales + o0 * a.groups;
     const uint32_t left = a.out_w - o0 < kOutputs ? static_cast<uint32_t>(a.out_w - o0) - 1 : kOutputs - 1;
-    uint32_t at[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads - 1; ++i) at[i] = code_place(i, block, left);
-    at[kLoads - 1] = scale_place(block, left);
+    for (int i = 0; i < 4; ++i)
+      __builtin_amdgcn_global_load_lds((const global_ptr*)(codes + code_place(i, block, left)),
+                                       (lds_ptr*)(room + (i * W + wave) * 1024), 16, 0, 0);
+    if constexpr (kWhole) {
+      __builtin_amdgcn_global_load_lds((const global_ptr*)(scales + scale_place(block, left)),
+                                       (lds_ptr*)(room + kStageScales + wave * 256), 4, 0, 0);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kLoads - 1; ++i)
-      __builtin_amdgcn_global_load_lds((const global_ptr*)(codes + at[i]), (lds_ptr*)(room + (i * W + wave) * 1024), 16, 0, 0);
-    __builtin_amdgcn_global_load_lds((const global_ptr*)(scales + at[kLoads - 1]),
-                                     (lds_ptr*)(room + kStageScales + wave * 256), 4, 0, 0);
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t row = min((tile0 + u * kTileStep) * 16 + i16, left);
+          const uint32_t group = min(block * kRow + (chunk + (kRow == 128 ? 8 * u : 0)) * 8 + 4 * h + g, a.groups - 1);
+          held.scale[u][h] = scales[row * a.groups + group];
+        }
+    }
   };
   f32x4 acc[kSums];
-  auto step = [&](const uint8_t* room, auto constant) __attribute__((always_inline)) {
+  auto step = [&](const uint8_t* room, const Held& held, auto constant) __attribute__((always_inline)) {
     constexpr int block = decltype(constant)::value;
     if (block == 0)
 #pragma unroll
@@ -461,9 +311,10 @@ void k_project_staged(const ProjectArgs a, uint32_t per_group) {
       for (int h = 0; h < 2; ++h) {
         const uint32_t piece = (chunk + 8 * c) * 8 + 4 * h + g, word = piece / 4;
         const u32x4 code = *reinterpret_cast<const u32x4*>(room + (row * kRow + (piece ^ i16)) * kGroupBytes);
-        const uint32_t scale =
-            *reinterpret_cast<const uint32_t*>(room + kStageScales + (row * kWords + (word ^ row % kWordSwizzle)) * 4);
-        const float by = scale_of(scale >> (8 * g) & 255u);
+        uint32_t scale = held.scale[u][h];
+        if constexpr (kWhole)
+          scale = *reinterpret_cast<const uint32_t*>(room + kStageScales + (row * kWords + (word ^ row % kWordSwizzle)) * 4) >> (8 * g) & 255u;
+        const float by = scale_of(scale);
 #pragma unroll
         for (int s = 0; s < 4; ++s) acc[to] = product(to_bf16(code[s], by), in[block][c][h][s], acc[to]);
       }
@@ -494,12 +345,12 @@ void k_project_staged(const ProjectArgs a, uint32_t per_group) {
       if (i16 < rows && o < a.out_w) store_four(y + static_cast<uint64_t>(first_row + i16) * a.out_w + o, sum, a.out_w - o, whole);
     }
   };
-  auto work = [&](uint8_t* room, uint32_t block) __attribute__((always_inline)) {
-    if (block == 0) step(room, std::integral_constant<int, 0>{});
+  auto work = [&](uint8_t* room, const Held& held, uint32_t block) __attribute__((always_inline)) {
+    if (block == 0) step(room, held, std::integral_constant<int, 0>{});
     if constexpr (kBlocks > 1)
-      if (block == 1) step(room, std::integral_constant<int, 1>{});
+      if (block == 1) step(room, held, std::integral_constant<int, 1>{});
     if constexpr (kBlocks > 2)
-      if (block == 2) step(room, std::integral_constant<int, 2>{});
+      if (block == 2) step(room, held, std::integral_constant<int, 2>{});
     if (block == kBlocks - 1)
 #pragma unroll
       for (int u = 0; u < kSums; ++u) reinterpret_cast<f32x4*>(room + kStageSums)[(u * W + wave) * 64 + lane] = acc[u];
@@ -515,9 +366,9 @@ void k_project_staged(const ProjectArgs a, uint32_t per_group) {
     __builtin_amdgcn_s_waitcnt(lds_wait((kStages - 2) * kLoads));
     meet();
     finish_before(project_stage<kBefore, kRoom>(), stage);
-    issue(project_stage<kBefore, kRoom>(), stage + kStages - 1);
+    issue(project_stage<kBefore, kRoom>(), ring[kBefore], stage + kStages - 1);
     __builtin_amdgcn_sched_barrier(0);
-    work(project_stage<kSlot, kRoom>(), kBlocks == kStages ? kSlot : stage % kBlocks);
+    work(project_stage<kSlot, kRoom>(), ring[kSlot], kBlocks == kStages ? kSlot : stage % kBlocks);
   };
   auto room_of = [&](uint32_t stage) {
     const uint32_t slot = stage % kStages;
@@ -525,11 +376,11 @@ void k_project_staged(const ProjectArgs a, uint32_t per_group) {
   };
   uint32_t stage = 0;
   if (total < kStages) {
-    issue(project_stage<0, kRoom>(), 0);
-    if (total > 1) issue(project_stage<1, kRoom>(), 1);
+    issue(project_stage<0, kRoom>(), ring[0], 0);
+    if (total > 1) issue(project_stage<1, kRoom>(), ring[1], 1);
   } else {
-    issue(project_stage<0, kRoom>(), 0);
-    issue(project_stage<1, kRoom>(), 1);
+    issue(project_stage<0, kRoom>(), ring[0], 0);
+    issue(project_stage<1, kRoom>(), ring[1], 1);
     __builtin_amdgcn_s_waitcnt(vm_wait(2 * kLoads));  // the inputs
     for (;;) {
       turn(std::integral_constant<int, 0>{}, stage++);
@@ -544,10 +395,63 @@ void k_project_staged(const ProjectArgs a, uint32_t per_group) {
     __builtin_amdgcn_s_waitcnt(lds_wait(0));
     meet();
     finish_before(room_of(stage + kStages - 1), stage);
-    work(room_of(stage), stage % kBlocks);
+    const uint32_t slot = stage % kStages;
+    Held held = {};
+    if constexpr (!kWhole)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t of[3] = {ring[0].scale[u / 2][u % 2], ring[1].scale[u / 2][u % 2], ring[2].scale[u / 2][u % 2]};
+        held.scale[u / 2][u % 2] = slot == 0 ? of[0] : slot == 1 ? of[1] : of[2];
+      }
+    work(room_of(stage), held, stage % kBlocks);
   }
   __syncthreads();
   finish(room_of(total - 1), count - 1);
+}
+
+// Few rows with more inputs than the staged kernel holds in registers: a workgroup per
+// 16 outputs, inputs and codes read as they are needed.
+template <class T, bool kPieces>
+__global__ __launch_bounds__(kProjectWaves * 64) void k_project_long(const ProjectArgs a) {
+  constexpr int W = kProjectWaves, kRows = columns_of<T>, kParts = sizeof(T) == 4 ? 3 : 1;
+  __shared__ f32x4 sums[W][64];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t i16 = lane % 16, g = lane / 16;
+  const uint32_t first_row = blockIdx.y * kRows, rows = min(a.rows - first_row, static_cast<uint32_t>(kRows));
+  const uint32_t column = min(i16, kParts * rows - 1), part = column / rows;
+  const T* x = static_cast<const T*>(a.x) + static_cast<uint64_t>(first_row + column % rows) * a.in_w;
+  const uint64_t o0 = static_cast<uint64_t>(blockIdx.x) * 16, output = min(o0 + i16, a.out_w - 1) * a.groups;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t group0 = wave * 4; group0 < a.groups; group0 += 4 * W) {
+    const uint32_t group = group0 + g, at = min(group, a.groups - 1);  // past the last: its inputs are zeros
+    const u32x4 code = load_stream(reinterpret_cast<const u32x4*>(a.codes) + output + at);
+    const float by = scale_of(a.scales[output + at]);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      float v[8];
+      load_eight<T, kPieces>(x, group * kGroup + 8 * s, a.in_w, v);
+      const Parts p = split(v);
+      acc = product(to_bf16(code[s], by), kParts == 1 || part == 0 ? p.part[0] : part == 1 ? p.part[1] : p.part[2], acc);
+    }
+  }
+  sums[wave][lane] = acc;
+  __syncthreads();
+  if (wave) return;
+  f32x4 sum = acc;
+#pragma unroll
+  for (int w = 1; w < W; ++w) sum = sum + sums[w][lane];
+  f32x4 all = sum;
+  if constexpr (kParts == 3) {  // the low parts' columns into the high ones'
+#pragma unroll
+    for (int p = 1; p < 3; ++p)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) all[e] = all[e] + __shfl(sum[e], lane + p * static_cast<int>(rows));
+  }
+  const uint64_t o = o0 + 4 * g;
+  if (i16 >= rows || o >= a.out_w) return;
+  T* y = static_cast<T*>(a.y) + (a.position ? *a.position * a.out_w : 0);
+  const bool whole = a.out_w % 4 == 0 && reinterpret_cast<uintptr_t>(a.y) % (4 * sizeof(T)) == 0;
+  store_four(y + static_cast<uint64_t>(first_row + i16) * a.out_w + o, all, a.out_w - o, whole);
 }
 
 // What loads to LDS take for inputs past the width.
@@ -752,39 +656,30 @@ void launch_project(hipStream_t s, const ProjectArgs& a) {
   const uint64_t row_tiles = ceil_div(a.rows, columns_of<T>);
   require(row_tiles <= 65535, "too many rows", DL_LENGTH_ERROR);
 #define I(n) std::integral_constant<int, n>{}
-  if (words && a.groups <= 384) {
-    auto run = [&](auto row, auto blocks) {
-      constexpr int kRow = decltype(row)::value, kBlocks = decltype(blocks)::value;
-      const uint64_t sets = ceil_div(a.out_w, 2048 / kRow), per_group = ceil_div(sets, 256);
-      const dim3 grid(static_cast<unsigned>(ceil_div(sets, per_group)), static_cast<unsigned>(row_tiles));
-      k_project_staged<T, kPieces, kRow, kBlocks><<<grid, kProjectWaves * 64, 0, s>>>(a, static_cast<uint32_t>(per_group));
-    };
-    if (a.groups <= 32)
-      run(I(32), I(1));
-    else if (a.groups <= 64)
-      run(I(64), I(1));
-    else if (a.groups <= 128)
-      run(I(128), I(1));
-    else if (a.groups <= 256)
-      run(I(128), I(2));
-    else
-      run(I(128), I(3));
+  if (a.groups > 384) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.out_w, 16)), static_cast<unsigned>(row_tiles));
+    k_project_long<T, kPieces><<<grid, kProjectWaves * 64, 0, s>>>(a);
     return;
   }
-  const uint64_t tiles = ceil_div(a.out_w, 16), slices = ceil_div(ceil_div(a.groups, 8), kProjectWaves);
-  auto run = [&](auto n, auto count, auto ahead, auto many) {
-    constexpr int kSlices = decltype(n)::value, kTiles = decltype(count)::value, kAhead = decltype(ahead)::value;
-    const uint64_t per_group = ceil_div(tiles, kSlices == 1 ? 512 : 256);
-    const dim3 grid(static_cast<unsigned>(ceil_div(tiles, per_group)), static_cast<unsigned>(row_tiles));
-    k_project<T, kPieces, kSlices, kTiles, kAhead, decltype(many)::value>
-        <<<grid, kProjectWaves * 64, 0, s>>>(a, static_cast<uint32_t>(per_group));
+  auto run = [&](auto row, auto blocks) {
+    constexpr int kRow = decltype(row)::value, kBlocks = decltype(blocks)::value;
+    const uint64_t sets = ceil_div(a.out_w, 2048 / kRow), per_group = ceil_div(sets, 256);
+    const dim3 grid(static_cast<unsigned>(ceil_div(sets, per_group)), static_cast<unsigned>(row_tiles));
+    if (words)
+      k_project_staged<T, kPieces, true, kRow, kBlocks><<<grid, kProjectWaves * 64, 0, s>>>(a, static_cast<uint32_t>(per_group));
+    else
+      k_project_staged<T, kPieces, false, kRow, kBlocks><<<grid, kProjectWaves * 64, 0, s>>>(a, static_cast<uint32_t>(per_group));
   };
-  if (slices == 1)
-    run(I(1), I(4), I(4), std::false_type{});
-  else if (slices == 2)
-    run(I(2), I(4), I(8), std::false_type{});
+  if (a.groups <= 32)
+    run(I(32), I(1));
+  else if (a.groups <= 64)
+    run(I(64), I(1));
+  else if (a.groups <= 128)
+    run(I(128), I(1));
+  else if (a.groups <= 256)
+    run(I(128), I(2));
   else
-    run(I(2), I(1), I(2), std::true_type{});
+    run(I(128), I(3));
 #undef I
 }
 
