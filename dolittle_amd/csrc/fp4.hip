@@ -13,29 +13,6 @@
 namespace dl::fp4 {
 namespace {
 
-// Eight consecutive elements of a row that has `width`, from `at` on; zeros past
-// the width.  Pieces: the row is whole 16-byte pieces.
-template <class T, bool kPieces>
-__device__ __forceinline__ void load_eight(const T* row, uint32_t at, uint32_t width, float (&x)[8]) {
-  if constexpr (kPieces) {
-    constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 8 / kPer; ++i) {
-      const u32x4 v = at + i * kPer < width ? *reinterpret_cast<const u32x4*>(row + at + i * kPer) : u32x4{};
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        if constexpr (sizeof(T) == 4)
-          x[i * kPer + e] = __uint_as_float(v[e]);
-        else
-          x[i * kPer + e] = e % 2 ? dl_bf16_hi(v[e / 2]) : dl_bf16_lo(v[e / 2]);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = at + e < width ? load_elem(row, at + e) : 0.0f;
-  }
-}
-
 __device__ __forceinline__ uint32_t largest_of(const float (&x)[8]) {
   uint32_t m = 0;
 #pragma unroll
@@ -150,9 +127,6 @@ __device__ __forceinline__ uint8_t* project_stage() {
   return room;
 }
 
-// s_waitcnt immediate: at most n vector-memory operations and no LDS operation
-// outstanding.
-constexpr unsigned lds_wait(unsigned n) { return vm_wait(n) & ~0x0f00u; }
 // A barrier alone: __syncthreads also waits for all loads to LDS, those of the stages
 // ahead among them.
 __device__ __forceinline__ void meet() {

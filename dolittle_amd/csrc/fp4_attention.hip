@@ -105,22 +105,27 @@ __device__ __forceinline__ uint64_t query_offset(const Args& a, uint32_t row, ui
 }
 
 // Eight consecutive query features as product operands; zeros past the width.
-template <class T>
+template <class T, bool kPieces>
 __device__ __forceinline__ void query_operands(const T* row, uint32_t at, uint32_t width, bool negative, u32x4* q) {
-  float x[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float v = at + e < width ? load_elem(row, at + e) : 0.0f;
-    x[e] = negative ? -v : v;
-  }
   if constexpr (sizeof(T) == 4) {
+    float x[8];
+    load_eight<T, kPieces>(row, at, width, x);
+#pragma unroll
+    for (float& v : x) v = negative ? -v : v;
     const Parts p = split(x);
 #pragma unroll
     for (int i = 0; i < 3; ++i) q[i] = p.part[i];
   } else {
+    const uint32_t signs = negative ? 0x80008000u : 0u;
+    if constexpr (kPieces) {
+      q[0] = (at < width ? *reinterpret_cast<const u32x4*>(row + at) : u32x4{}) ^ signs;
+    } else {
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-      q[0][w] = __float_as_uint(x[2 * w]) >> 16 | (__float_as_uint(x[2 * w + 1]) & 0xffff0000u);
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t f = at + 2 * w, lo = f < width ? row[f] : 0u, hi = f + 1 < width ? row[f + 1] : 0u;
+        q[0][w] = (lo | hi << 16) ^ signs;
+      }
+    }
   }
 }
 
@@ -143,19 +148,6 @@ __device__ __forceinline__ void share_operands(const f32x4 (&p)[2], u32x4 (&b)[k
   }
 }
 
-// N words of codes from a byte offset past a base that the wavefront shares.
-template <int N>
-__device__ __forceinline__ void load_codes(const uint8_t* base, uint32_t offset, uint32_t* w) {
-  if constexpr (N == 1) {
-    w[0] = *reinterpret_cast<const uint32_t*>(base + offset);
-  } else {
-    typedef uint32_t Words __attribute__((ext_vector_type(N)));
-    const Words v = *reinterpret_cast<const Words*>(base + offset);
-#pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = v[i];
-  }
-}
-
 // D features (64, 128 or 256, at least the width) and storage T of query and output.
 template <class T, int D>
 struct Tile {
@@ -167,11 +159,19 @@ struct Tile {
   static constexpr int kValueWords = C < 8 ? 1 : C / 8;       // D = 64: four codes, the lower half of a word
 };
 
-template <class T, int D>
+// A step's codes of one wavefront: 32 keys, then their values, D / 2 bytes each.
+// Objects apart, so that the compiler sees no use of loads in flight.
+constexpr int kRing = 3;
+template <int D, int kSlot>
+__device__ __forceinline__ uint8_t* step_room() {
+  __shared__ __align__(1024) uint8_t room[kWaves * 32 * D];
+  return room;
+}
+
+template <class T, int D, bool kPieces>
 __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
   using S = Tile<T, D>;
   constexpr int C = S::C, kParts = S::kParts;
-  __shared__ f32x4 room[kWaves / 2][C][64];
   __shared__ float2 stats[kWaves][16];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t i16 = lane % 16, g = lane / 16;
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
   u32x4 q[S::kSteps][kParts];
 #pragma unroll
   for (int s = 0; s < S::kSteps; ++s)
-    query_operands(static_cast<const T*>(a.query) + query_offset(a, row, kvh), g * (D / 4) + 8 * s, a.width, scale < 0.0f, q[s]);
+    query_operands<T, kPieces>(static_cast<const T*>(a.query) + query_offset(a, row, kvh), g * (D / 4) + 8 * s, a.width, scale < 0.0f, q[s]);
 
   const uint64_t head = (static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.capacity;
   const uint32_t row_bytes = a.groups * kGroupBytes;
@@ -203,56 +203,70 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
   const uint8_t* key_scales = a.key_scales + head * a.groups;
   const uint8_t* value_scales = a.value_scales + head * a.groups;
 
-  // A lane's features past the row's last group repeat its last bytes: the query has
-  // zeros there, and such features of the output are not stored.
-  uint32_t key_words[2][S::kKeyWords], key_bytes[2][S::kKeyScales], value_words[8][S::kValueWords], value_bytes[8];
-  constexpr uint32_t kUnit = D < 128 ? 8 : kGroupBytes;  // of a key's codes, within a group
-  uint32_t key_at[S::kKeyWords * 4 / kUnit];
-#pragma unroll
-  for (uint32_t x = 0; x < S::kKeyWords * 4 / kUnit; ++x) key_at[x] = min(g * (D / 8) + x * kUnit, row_bytes - kUnit);
-  const uint32_t value_at = min(i16 * (C / 2), row_bytes - C / 2), value_group = min(i16 * C / kGroup, a.groups - 1);
-  auto load = [&](uint32_t at) {
+  // Codes go through LDS of the wavefront's own, 1 KiB a load, two steps ahead; scale
+  // bytes to registers as far ahead.  Features past the row's last group repeat it: the
+  // query has zeros there, and such features of the output are not stored.  Piece p of a
+  // key's codes lies at p ^ key / 8, so that the keys of an operand lie in distinct banks.
+  constexpr uint32_t P = D / 32, kRowBytes = D / 2, kHalf = 16 * D;  // pieces of a key; bytes of 32
+  const uint32_t value_group = min(i16 * C / kGroup, a.groups - 1);
+  struct Scales {
+    uint32_t key[2][S::kKeyScales], value[8];
+  };
+  Scales ring[kRing];
+  auto load = [&](uint8_t* room, Scales& to, uint32_t at) __attribute__((always_inline)) {
     const uint32_t last = n - 1 - at;  // rows past the last repeat it: nobody sees them
     const uint8_t* kc = key_codes + static_cast<uint64_t>(at) * row_bytes;
-    const uint8_t* ks = key_scales + static_cast<uint64_t>(at) * a.groups;
     const uint8_t* vc = value_codes + static_cast<uint64_t>(at) * row_bytes;
+    const uint8_t* ks = key_scales + static_cast<uint64_t>(at) * a.groups;
     const uint8_t* vs = value_scales + static_cast<uint64_t>(at) * a.groups;
+    uint8_t* mine = room + wave * (2 * kHalf);
+#pragma unroll
+    for (uint32_t x = 0; x < kHalf / 1024; ++x) {
+      const uint32_t slot = x * 64 + lane, key = slot / P, piece = min(slot % P ^ key / 8 % P, a.groups - 1);
+      const uint32_t from = min(key, last) * row_bytes + piece * kGroupBytes;
+      __builtin_amdgcn_global_load_lds((const global_ptr*)(kc + from), (lds_ptr*)(mine + x * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const global_ptr*)(vc + from), (lds_ptr*)(mine + kHalf + x * 1024), 16, 0, 0);
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint32_t k = min(8 * (i16 / 4) + 4 * u + i16 % 4, last);
 #pragma unroll
-      for (uint32_t x = 0; x < S::kKeyWords * 4 / kUnit; ++x) load_codes<kUnit / 4>(kc, k * row_bytes + key_at[x], key_words[u] + x * kUnit / 4);
-#pragma unroll
-      for (int h = 0; h < S::kKeyScales; ++h) key_bytes[u][h] = ks[k * a.groups + min(g * (D / 4) / kGroup + h, a.groups - 1)];
+      for (int h = 0; h < S::kKeyScales; ++h) to.key[u][h] = ks[k * a.groups + min(g * (D / 4) / kGroup + h, a.groups - 1)];
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t k = min(8 * g + e, last);
-      if constexpr (C == 4)
-        value_words[e][0] = *reinterpret_cast<const uint16_t*>(vc + k * row_bytes + value_at);
-      else
-        load_codes<S::kValueWords>(vc, k * row_bytes + value_at, value_words[e]);
-      value_bytes[e] = vs[k * a.groups + value_group];
-    }
+    for (int e = 0; e < 8; ++e) to.value[e] = vs[min(8 * g + e, last) * a.groups + value_group];
   };
+  constexpr int kLoads = 2 * kHalf / 1024 + 2 * S::kKeyScales + 8;
 
   f32x4 o[C];
   float top = -INFINITY, from = 0.0f, most_sum = -1.0f, sum = 0.0f;
 #pragma unroll
   for (int j = 0; j < C; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  uint32_t step = begin + wave;
-  if (step < end) load(steps.key(step));
-  for (; step < end; step += kWaves) {
-    const uint32_t at = steps.key(step);
+  auto work = [&](const uint8_t* room, const Scales& by, uint32_t at) __attribute__((always_inline)) {
+    const uint8_t* keys = room + wave * (2 * kHalf);
     // Scores of the lane's row and the keys at + 8 g + 4 u + r.
     f32x4 p[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+      const uint32_t key = 8 * (i16 / 4) + 4 * u + i16 % 4, swizzle = i16 / 4 % P;
+      uint32_t words[S::kKeyWords];
+      if constexpr (D == 64) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(keys + key * kRowBytes + (g / 2 ^ swizzle) * 16 + g % 2 * 8);
+        words[0] = v.x;
+        words[1] = v.y;
+      } else {
+#pragma unroll
+        for (int h = 0; h < D / 128; ++h) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(keys + key * kRowBytes + ((g * (D / 128) + h) ^ swizzle) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) words[4 * h + e] = v[e];
+        }
+      }
       p[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < S::kSteps; ++s) {
-        const u32x4 k = to_bf16(key_words[u][s], scale_of(key_bytes[u][s * S::kKeyScales / S::kSteps]));
+        const u32x4 k = to_bf16(words[s], scale_of(by.key[u][s * S::kKeyScales / S::kSteps]));
 #pragma unroll
         for (int i = 0; i < kParts; ++i) p[u] = product(k, q[s][i], p[u]);
       }
@@ -260,11 +274,19 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
     uint32_t words[8][S::kValueWords], bytes[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      bytes[e] = value_bytes[e];
-#pragma unroll
-      for (int w = 0; w < S::kValueWords; ++w) words[e][w] = value_words[e][w];
+      bytes[e] = by.value[e];
+      const uint32_t byte = i16 * (C / 2);  // of the key's codes
+      const uint8_t* from = keys + kHalf + (8 * g + e) * kRowBytes + (byte / 16 ^ g % P) * 16 + byte % 16;
+      if constexpr (C == 4) {
+        words[e][0] = *reinterpret_cast<const uint16_t*>(from);
+      } else if constexpr (C == 8) {
+        words[e][0] = *reinterpret_cast<const uint32_t*>(from);
+      } else {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(from);
+        words[e][0] = v.x;
+        words[e][1] = v.y;
+      }
     }
-    load(steps.key(min(step + kWaves, end - 1)));
 
     const bool masked = at + kKeys > least.end || (a.window && at < most.low && at + kKeys > a.sinks);
     auto hide = [&](f32x4 (&v)[2], float value) {
@@ -351,10 +373,35 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
 #pragma unroll
       for (int i = 0; i < kParts; ++i) o[j] = product(v, shares[i], o[j]);
     }
+  };
+  // Loads past the last step repeat it; none lies under a condition, and the loop is left
+  // at its end alone: the compiler would wait for all loads in flight.
+  auto turn = [&](auto slot, uint32_t step) __attribute__((always_inline)) {
+    constexpr int kSlot = decltype(slot)::value, kNext = (kSlot + kRing - 1) % kRing;
+    __builtin_amdgcn_s_waitcnt(lds_wait((kRing - 2) * kLoads));  // this step's codes; the room loaded next is read
+    asm volatile("" ::: "memory");
+    load(step_room<D, kNext>(), ring[kNext], steps.key(min(step + (kRing - 1) * kWaves, end - 1)));
+    __builtin_amdgcn_sched_barrier(0);
+    if (step < end) work(step_room<D, kSlot>(), ring[kSlot], steps.key(step));
+  };
+  uint32_t step = begin + wave;
+  if (step < end) {
+    load(step_room<D, 0>(), ring[0], steps.key(step));
+    __builtin_amdgcn_sched_barrier(0);
+    load(step_room<D, 1>(), ring[1], steps.key(min(step + kWaves, end - 1)));
+    __builtin_amdgcn_sched_barrier(0);
+    for (; step < end; step += kRing * kWaves) {
+      turn(std::integral_constant<int, 0>{}, step);
+      turn(std::integral_constant<int, 1>{}, step + kWaves);
+      turn(std::integral_constant<int, 2>{}, step + 2 * kWaves);
+    }
   }
   sum = group_sum(sum);
 
   // Join the wavefronts: the upper half into the lower, and so on.
+  __syncthreads();  // nothing reads or loads the steps' rooms any more
+  f32x4 (*room)[C][64] = reinterpret_cast<f32x4 (*)[C][64]>(step_room<D, 0>());
+  static_assert(kWaves / 2 * C * 1024 <= kWaves * 32 * D, "joined outputs outgrow a room");
 #pragma unroll
   for (int half = kWaves / 2; half; half /= 2) {
     if (wave >= half && wave < 2 * half) {
@@ -400,43 +447,71 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
     }
 }
 
-// Joins the ranges of one row: a wavefront, D / 64 features a lane.
-template <class T, int D>
+// Joins the ranges of one row, W wavefronts a row.  D / 4 lanes hold a row of a range,
+// four features each, so a wavefront reads 256 / D ranges at a time.  Sums are read
+// before the maxima say how much of them counts: one wait and not two.
+template <class T, int D, int W>
 __global__ __launch_bounds__(kThreads) void k_join(const Args a) {
-  constexpr int kPer = D / 64;
+  constexpr uint32_t kLanes = D / 4, kAtOnce = W * 64 / kLanes, kAhead = 4, kTasks = kWaves / W;
+  __shared__ f32x4 room[kWaves][64];
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const uint64_t tasks = static_cast<uint64_t>(a.kv_heads) * a.all_rows;
-  for (uint64_t task = static_cast<uint64_t>(blockIdx.x) * kWaves + wave; task < tasks; task += static_cast<uint64_t>(gridDim.x) * kWaves) {
-    const uint32_t row = static_cast<uint32_t>(task % a.all_rows), kvh = static_cast<uint32_t>(task / a.all_rows);
-    const uint32_t in_seq = row % a.seq_rows, tile = in_seq / 16, n = length_of(a, row / a.seq_rows);
-    const uint32_t last = min(tile * 16 + 15, a.seq_rows - 1);
-    const Sight sight = sight_of(a, n, in_seq / a.group);
-    const Steps steps(a, sight_of(a, n, tile * 16 / a.group), sight_of(a, n, last / a.group));
-    const uint32_t each = range_steps(steps.count, a.splits);
-    const uint32_t ranges = steps.count ? (steps.count + each - 1) / each : 0;
-    const uint64_t stride = tasks;
-    float top = -INFINITY;
-    for (uint32_t r = 0; r < ranges; ++r) top = fmaxf(top, a.part[r * stride + task].x);
-    const float from = reference_of(top);
-    float sum = 0.0f, acc[kPer] = {};
-    for (uint32_t r = 0; r < ranges; ++r) {
-      const float2 part = a.part[r * stride + task];
-      const float share = exp2_of(part.x - from);
-      sum = fma_rn(share, part.y, sum);
-      const float* sums = a.sums + (r * stride + task) * a.pitch;
+  const uint32_t tasks = a.kv_heads * a.all_rows, task = blockIdx.x * kTasks + wave / W;
+  if (task >= tasks) return;  // wavefronts of one row end together
+  const uint32_t row = task % a.all_rows, kvh = task / a.all_rows;
+  const uint32_t in_seq = row % a.seq_rows, tile = in_seq / 16, n = length_of(a, row / a.seq_rows);
+  const uint32_t f = lane % kLanes * 4, first = wave % W * (64 / kLanes) + lane / kLanes;
+  const float* sums = a.sums + (f < a.pitch ? f : 0);
+  f32x4 ahead[kAhead];
 #pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        if (lane * kPer + e < a.pitch) acc[e] = fma_rn(share, sums[lane * kPer + e], acc[e]);
-    }
-    T* out = static_cast<T*>(a.out) + query_offset(a, row, kvh);
-#pragma unroll
-    for (int e = 0; e < kPer; ++e)
-      if (lane * kPer + e < a.width) store_elem(out, lane * kPer + e, sight.end ? acc[e] / sum : 0.0f);
+  for (uint32_t m = 0; m < kAhead; ++m)
+    ahead[m] = *reinterpret_cast<const f32x4*>(sums + (static_cast<uint64_t>(min(m * kAtOnce + first, a.splits - 1)) * tasks + task) * a.pitch);
+  const Sight sight = sight_of(a, n, in_seq / a.group);
+  const Steps steps(a, sight_of(a, n, tile * 16 / a.group), sight_of(a, n, min(tile * 16 + 15, a.seq_rows - 1) / a.group));
+  const uint32_t each = range_steps(steps.count, a.splits), ranges = steps.count ? (steps.count + each - 1) / each : 0;
+  auto part = [&](uint32_t r) { return a.part[static_cast<uint64_t>(r) * tasks + task]; };
+  const float2 mine = lane < ranges ? part(lane) : make_float2(-INFINITY, 0.0f);
+  float top = mine.x;
+  for (uint32_t r = lane + 64; r < ranges; r += 64) top = fmaxf(top, part(r).x);
+  const float from = reference_of(wave_max(top));
+  float sum = exp2_of(mine.x - from) * mine.y;
+  for (uint32_t r = lane + 64; r < ranges; r += 64) {
+    const float2 p = part(r);
+    sum = fma_rn(exp2_of(p.x - from), p.y, sum);
   }
+#pragma unroll
+  for (int off = 32; off; off /= 2) sum = sum + __shfl_xor(sum, off);
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto add = [&](uint32_t r, const f32x4& v) {
+    const float share = exp2_of(part(r).x - from);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fma_rn(share, v[e], acc[e]);
+  };
+#pragma unroll
+  for (uint32_t m = 0; m < kAhead; ++m)
+    if (m * kAtOnce + first < ranges) add(m * kAtOnce + first, ahead[m]);
+  for (uint32_t r = kAhead * kAtOnce + first; r < ranges; r += kAtOnce)
+    add(r, *reinterpret_cast<const f32x4*>(sums + (static_cast<uint64_t>(r) * tasks + task) * a.pitch));
+#pragma unroll
+  for (uint32_t off = kLanes; off < 64; off *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = acc[e] + __shfl_xor(acc[e], off);
+  if constexpr (W > 1) {
+    room[wave][lane] = acc;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) acc = acc + room[w][lane];
+  }
+  if (lane >= kLanes) return;
+  T* out = static_cast<T*>(a.out) + query_offset(a, row, kvh);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (f + e < a.width) store_elem(out, f + e, sight.end ? acc[e] / sum : 0.0f);
 }
 
 // ------------------------------------------------------------------- the host
 constexpr uint64_t kMostBlocks = (1u << 23) - 8;
+constexpr uint32_t kFewRanges = 8;
 
 uint64_t times(uint64_t x, uint64_t y, uint64_t most, const char* what) {
   require(y == 0 || x <= most / y, what, DL_LENGTH_ERROR);
@@ -469,7 +544,7 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks) {
   constexpr const char* kRows = "too many query rows";
   a.seq_rows = static_cast<uint32_t>(times(a.rows, a.group, 1u << 30, kRows));
   a.all_rows = static_cast<uint32_t>(times(a.seq_rows, a.batch, 1u << 30, kRows));
-  times(a.all_rows, a.kv_heads, 1u << 30, kRows);
+  times(a.all_rows, a.kv_heads, 1u << 23, kRows);  // workgroups of the join
   a.tiles = static_cast<uint32_t>(ceil_div(a.seq_rows, 16));
   a.pitch = (a.width + 3) / 4 * 4;
   // Most steps that a row tile can see, and ranges for two workgroups a compute unit.
@@ -477,7 +552,7 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks) {
   if (a.window) keys = std::min<uint64_t>(keys, uint64_t{a.window} + a.sinks + 16 + 3 * kKeys);
   const uint64_t rounds = ceil_div(keys, kKeys * kWaves);
   const uint64_t tasks = times(times(a.batch, a.kv_heads, kMostBlocks, "too many workgroups"), a.tiles, kMostBlocks, "too many workgroups");
-  a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(ceil_div(rounds, 2), 512 / tasks)));
+  a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(ceil_div(rounds, 2), ceil_div(1024, tasks))));
   const uint64_t groups = times(uint64_t{a.batch} * a.kv_heads, a.splits, kMostBlocks, "too many workgroups");
   l.blocks = static_cast<uint32_t>(times(ceil_div(groups, 8) * 8, a.tiles, kMostBlocks, "too many workgroups"));
   if (a.splits > 1) {
@@ -489,22 +564,27 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks) {
 }
 
 template <class T, int D>
-void launch(hipStream_t s, const Layout& l) {
-  k_attend<T, D><<<l.blocks, kThreads, 0, s>>>(l.args);
-  if (l.args.splits > 1) {
-    const uint64_t blocks = ceil_div(uint64_t{l.args.kv_heads} * l.args.all_rows, kWaves);
-    k_join<T, D><<<static_cast<unsigned>(std::min<uint64_t>(blocks, 1u << 20)), kThreads, 0, s>>>(l.args);
-  }
+void launch(hipStream_t s, const Layout& l, bool pieces) {
+  if (pieces)
+    k_attend<T, D, true><<<l.blocks, kThreads, 0, s>>>(l.args);
+  else
+    k_attend<T, D, false><<<l.blocks, kThreads, 0, s>>>(l.args);
+  // A workgroup per row where there are many ranges, else a wavefront.
+  const uint64_t tasks = uint64_t{l.args.kv_heads} * l.args.all_rows;
+  if (l.args.splits > kFewRanges)
+    k_join<T, D, kWaves><<<static_cast<unsigned>(tasks), kThreads, 0, s>>>(l.args);
+  else if (l.args.splits > 1)
+    k_join<T, D, 1><<<static_cast<unsigned>(ceil_div(tasks, kWaves)), kThreads, 0, s>>>(l.args);
 }
 
 template <class T>
-void launch_width(hipStream_t s, const Layout& l) {
+void launch_width(hipStream_t s, const Layout& l, bool pieces) {
   if (l.args.width <= 64)
-    launch<T, 64>(s, l);
+    launch<T, 64>(s, l, pieces);
   else if (l.args.width <= 128)
-    launch<T, 128>(s, l);
+    launch<T, 128>(s, l, pieces);
   else
-    launch<T, 256>(s, l);
+    launch<T, 256>(s, l, pieces);
 }
 
 }  // namespace
@@ -548,10 +628,11 @@ int dl_attention_fp4(dl_queue* queue, int dtype, const dl_batch_shape* shape, co
     a.out = output;
     a.part = static_cast<float2*>(workspace);
     a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + l.part_bytes);
+    const bool pieces = (shape->width * (dtype == DL_BF16 ? 2 : 4)) % 16 == 0 && aligned(query);
     if (dtype == DL_BF16)
-      launch_width<uint16_t>(queue->stream, l);
+      launch_width<uint16_t>(queue->stream, l, pieces);
     else
-      launch_width<float>(queue->stream, l);
+      launch_width<float>(queue->stream, l, pieces);
     dl::check_launch(queue, "attention_fp4");
   });
 }
