@@ -110,4 +110,21 @@ __device__ __forceinline__ void load_eight(const T* row, uint32_t at, uint32_t w
 // outstanding.
 constexpr unsigned lds_wait(unsigned n) { return vm_wait(n) & ~0x0f00u; }
 
+// Four consecutive outputs of a row.
+template <class T>
+__device__ __forceinline__ void store_four(T* to, const f32x4& v, uint64_t left, bool whole) {
+  struct alignas(4 * sizeof(T)) Four {
+    T v[4];
+  } four;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) store_elem(four.v, e, v[e]);
+  if (whole && left >= 4) {
+    *reinterpret_cast<Four*>(to) = four;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (static_cast<uint64_t>(e) < left) to[e] = four.v[e];
+  }
+}
+
 }  // namespace dl::fp4

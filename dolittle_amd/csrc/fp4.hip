@@ -83,23 +83,6 @@ __device__ __forceinline__ f32x4 product(const u32x4& a, const u32x4& b, const f
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Four consecutive outputs of a row.
-template <class T>
-__device__ __forceinline__ void store_four(T* to, const f32x4& v, uint64_t left, bool whole) {
-  struct alignas(4 * sizeof(T)) Four {
-    T v[4];
-  } four;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) store_elem(four.v, e, v[e]);
-  if (whole && left >= 4) {
-    *reinterpret_cast<Four*>(to) = four;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (static_cast<uint64_t>(e) < left) to[e] = four.v[e];
-  }
-}
-
 // Few rows (16 of BF16, 5 of FP32 as three exact parts in columns of their own):
 // bound by the weights' stream.  Eight wavefronts cut the inputs, 256 at a time.
 // Inputs are the products' second operands; 16 outputs' codes are first operands, a

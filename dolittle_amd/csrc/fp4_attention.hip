@@ -7,10 +7,10 @@
 // the slots j <= p, under a window only j > p - window or j < sinks.  A row
 // without a key is zeros.
 //
-// Split.  A workgroup takes 16 of a sequence's rows of one KV head (new rows times
-// the heads of the group) and a range of the steps of 32 keys that any of them
-// sees; its wavefronts take every fourth step, codes straight from memory into
-// registers, a step ahead.  Ranges leave their maximum, sum and unnormalised
+// Split.  A workgroup takes 16 or 32 of a sequence's rows of one KV head (new rows
+// times the heads of the group) and a range of the steps of 32 keys that any of them
+// sees; its wavefronts take every fourth step, whose codes come through LDS rooms of
+// their own, two steps ahead.  Ranges leave their maximum, sum and unnormalised
 // output, which k_join joins; a single range writes the output itself.
 //
 // Operands.  A lane takes D / 4 neighbouring features of a key's codes, one to two
@@ -47,7 +47,8 @@ struct Args {
   float2* part;  // [range][kv head][row]: maximum, sum
   float* sums;   // [range][kv head][row][pitch]: unnormalised output
   uint32_t batch, rows, q_heads, kv_heads, group, width, groups, capacity, window, sinks;
-  uint32_t seq_rows, all_rows, splits, tiles, pitch;
+  uint32_t seq_rows, all_rows, splits, tiles, tile_rows, pitch;
+  bool whole_out;  // output rows in fours of whole alignment
 };
 
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
@@ -63,6 +64,17 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 __device__ __forceinline__ f32x4 product(const u32x4& a, const u32x4& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// Products' results are there 8 instructions after the last of them.  The compiler counts
+// these along straight code and, behind a branch, has read one 3 later: a wrong score.
+// So they are waited for here, before any branch.
+template <int N>
+__device__ __forceinline__ void settle(f32x4 (&p)[N][2]) {
+  static_assert(N == 1 || N == 2);
+  if constexpr (N == 1)
+    asm volatile("s_nop 7" : "+v"(p[0][0]), "+v"(p[0][1]));
+  else
+    asm volatile("s_nop 7" : "+v"(p[0][0]), "+v"(p[0][1]), "+v"(p[1][0]), "+v"(p[1][1]));
 }
 
 __device__ __forceinline__ uint32_t length_of(const Args& a, uint32_t b) {
@@ -168,8 +180,10 @@ __device__ __forceinline__ uint8_t* step_room() {
   return room;
 }
 
-template <class T, int D, bool kPieces>
-__global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
+// Of two tiles of rows a wavefront holds twice the queries and outputs: left to itself
+// the compiler takes 300 registers, one workgroup a unit, 91 us where this takes 62.
+template <class T, int D, bool kPieces, int QT>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) void k_attend(const Args a) {
   using S = Tile<T, D>;
   constexpr int C = S::C, kParts = S::kParts;
   __shared__ float2 stats[kWaves][16];
@@ -181,8 +195,10 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
   if (task >= a.batch * a.kv_heads * a.splits) return;
   const uint32_t range = task % a.splits, kvh = task / a.splits % a.kv_heads, b = task / a.splits / a.kv_heads;
   const uint32_t n = length_of(a, b);
-  const uint32_t first = tile * 16, count = min(a.seq_rows - first, 16u);
-  const Sight sight = sight_of(a, n, (first + min(i16, count - 1)) / a.group);
+  const uint32_t first = tile * 16 * QT, count = min(a.seq_rows - first, 16u * QT);
+  Sight sight[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) sight[t] = sight_of(a, n, (first + min(16 * t + i16, count - 1)) / a.group);
   const Sight least = sight_of(a, n, first / a.group), most = sight_of(a, n, (first + count - 1) / a.group);
   const Steps steps(a, least, most);
   const uint32_t each = range_steps(steps.count, a.splits);
@@ -190,11 +206,14 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
   if (begin >= end && range > 0) return;
 
   const float scale = *a.scale, factor = fabsf(scale) * kLog2e;
-  const uint32_t row = b * a.seq_rows + first + min(i16, count - 1);  // the lane's
-  u32x4 q[S::kSteps][kParts];
+  auto row_of = [&](int t) { return b * a.seq_rows + first + min(16 * t + i16, count - 1); };  // the lane's
+  u32x4 q[QT][S::kSteps][kParts];
 #pragma unroll
-  for (int s = 0; s < S::kSteps; ++s)
-    query_operands<T, kPieces>(static_cast<const T*>(a.query) + query_offset(a, row, kvh), g * (D / 4) + 8 * s, a.width, scale < 0.0f, q[s]);
+  for (int t = 0; t < QT; ++t)
+#pragma unroll
+    for (int s = 0; s < S::kSteps; ++s)
+      query_operands<T, kPieces>(static_cast<const T*>(a.query) + query_offset(a, row_of(t), kvh), g * (D / 4) + 8 * s, a.width,
+                                 scale < 0.0f, q[t][s]);
 
   const uint64_t head = (static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.capacity;
   const uint32_t row_bytes = a.groups * kGroupBytes;
@@ -238,15 +257,23 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
   };
   constexpr int kLoads = 2 * kHalf / 1024 + 2 * S::kKeyScales + 8;
 
-  f32x4 o[C];
-  float top = -INFINITY, from = 0.0f, most_sum = -1.0f, sum = 0.0f;
+  f32x4 o[QT][C];
+  float top[QT], from[QT], most_sum[QT], sum[QT];
 #pragma unroll
-  for (int j = 0; j < C; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t = 0; t < QT; ++t) {
+    top[t] = -INFINITY;
+    from[t] = sum[t] = 0.0f;
+    most_sum[t] = -1.0f;
+#pragma unroll
+    for (int j = 0; j < C; ++j) o[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
 
   auto work = [&](const uint8_t* room, const Scales& by, uint32_t at) __attribute__((always_inline)) {
     const uint8_t* keys = room + wave * (2 * kHalf);
-    // Scores of the lane's row and the keys at + 8 g + 4 u + r.
-    f32x4 p[2];
+    // No branch, which the && and || would be, lies between products and their use.
+    const bool masked = (at + kKeys > least.end) | ((a.window != 0) & (at < most.low) & (at + kKeys > a.sinks));
+    // Scores of the lane's rows and the keys at + 8 g + 4 u + r.
+    f32x4 p[QT][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint32_t key = 8 * (i16 / 4) + 4 * u + i16 % 4, swizzle = i16 / 4 % P;
@@ -263,14 +290,18 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
           for (int e = 0; e < 4; ++e) words[4 * h + e] = v[e];
         }
       }
-      p[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int t = 0; t < QT; ++t) p[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < S::kSteps; ++s) {
         const u32x4 k = to_bf16(words[s], scale_of(by.key[u][s * S::kKeyScales / S::kSteps]));
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) p[u] = product(k, q[s][i], p[u]);
+        for (int i = 0; i < kParts; ++i)
+#pragma unroll
+          for (int t = 0; t < QT; ++t) p[t][u] = product(k, q[t][s][i], p[t][u]);
       }
     }
+    settle(p);
     uint32_t words[8][S::kValueWords], bytes[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -288,44 +319,48 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
       }
     }
 
-    const bool masked = at + kKeys > least.end || (a.window && at < most.low && at + kKeys > a.sinks);
-    auto hide = [&](f32x4 (&v)[2], float value) {
+    u32x4 shares[QT][kParts];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int t = 0; t < QT; ++t) {
+      auto hide = [&](f32x4 (&v)[2], float value) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t j = at + 8 * g + 4 * u + r;
-          if (j >= sight.end || (j < sight.low && j >= a.sinks)) v[u][r] = value;
-        }
-    };
-    f32x4 e[2];
-    auto weigh = [&] {
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t j = at + 8 * g + 4 * u + r;
+            if (j >= sight[t].end || (j < sight[t].low && j >= a.sinks)) v[u][r] = value;
+          }
+      };
+      f32x4 e[2];
+      auto weigh = [&] {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) e[u][r] = exp2_of(fma_rn(p[u][r], factor, from));
-      if (rare(masked)) hide(e, 0.0f);
-      return ((e[0][0] + e[0][1]) + (e[0][2] + e[0][3])) + ((e[1][0] + e[1][1]) + (e[1][2] + e[1][3]));
-    };
-    float s = weigh();
-    if (rare(__any(!(s <= most_sum)))) {
-      // Each row by itself: what another row sees changes no bit of this one.
-      const bool rises = group_max(s <= most_sum ? 0.0f : 1.0f) > 0.0f;
-      if (masked) hide(p, -INFINITY);
-      float high = -INFINITY;
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) high = fmaxf(high, fmaxf(fmaxf(p[u][0], p[u][1]), fmaxf(p[u][2], p[u][3])));
-      const float highest = group_max(high) * factor, raised = rises ? fmaxf(top, highest) : top;
-      const float less = top == -INFINITY ? 1.0f : exp2_of(top - raised);
-      top = raised;
-      from = -reference_of(raised);
-      most_sum = raised == -INFINITY ? -1.0f : kMostSum;
-      sum = sum * less;
+          for (int r = 0; r < 4; ++r) e[u][r] = exp2_of(fma_rn(p[t][u][r], factor, from[t]));
+        if (rare(masked)) hide(e, 0.0f);
+        return ((e[0][0] + e[0][1]) + (e[0][2] + e[0][3])) + ((e[1][0] + e[1][1]) + (e[1][2] + e[1][3]));
+      };
+      float s = weigh();
+      if (rare(__any(!(s <= most_sum[t])))) {
+        // Each row by itself: what another row sees changes no bit of this one.
+        const bool rises = group_max(s <= most_sum[t] ? 0.0f : 1.0f) > 0.0f;
+        if (masked) hide(p[t], -INFINITY);
+        float high = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < C; ++j) o[j] = o[j] * less;
-      s = weigh();
+        for (int u = 0; u < 2; ++u) high = fmaxf(high, fmaxf(fmaxf(p[t][u][0], p[t][u][1]), fmaxf(p[t][u][2], p[t][u][3])));
+        const float highest = group_max(high) * factor, raised = rises ? fmaxf(top[t], highest) : top[t];
+        const float less = top[t] == -INFINITY ? 1.0f : exp2_of(top[t] - raised);
+        top[t] = raised;
+        from[t] = -reference_of(raised);
+        most_sum[t] = raised == -INFINITY ? -1.0f : kMostSum;
+        sum[t] = sum[t] * less;
+#pragma unroll
+        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * less;
+        s = weigh();
+      }
+      sum[t] = sum[t] + s;
+      share_operands<kParts>(e, shares[t]);
     }
-    sum = sum + s;
 
     if (rare(masked)) {
       // A NaN group of a key that only some rows see must not reach the others
@@ -342,17 +377,18 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
 #pragma unroll 1
         for (uint32_t k = 0; k < kKeys && at + k < n; ++k) {
           const uint32_t j = at + k;
-          if (j >= sight.end || (j < sight.low && j >= a.sinks)) continue;
 #pragma unroll
-          for (int t = 0; t < C; ++t)
+          for (int t = 0; t < QT; ++t) {
+            if (j >= sight[t].end || (j < sight[t].low && j >= a.sinks)) continue;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (vs[k * a.groups + min(((4 * g + r) * C + t) / kGroup, a.groups - 1)] == kNanScale) o[t][r] = NAN;
+            for (int x = 0; x < C; ++x)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (vs[k * a.groups + min(((4 * g + r) * C + x) / kGroup, a.groups - 1)] == kNanScale) o[t][x][r] = NAN;
+          }
         }
       }
     }
-    u32x4 shares[kParts];
-    share_operands<kParts>(e, shares);
     uint32_t values[8][C / 2];  // pairs of features
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -371,7 +407,9 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
       for (int w = 0; w < 4; ++w)
         v[w] = __builtin_amdgcn_perm(values[2 * w + 1][j / 2], values[2 * w][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-      for (int i = 0; i < kParts; ++i) o[j] = product(v, shares[i], o[j]);
+      for (int i = 0; i < kParts; ++i)
+#pragma unroll
+        for (int t = 0; t < QT; ++t) o[t][j] = product(v, shares[t][i], o[t][j]);
     }
   };
   // Loads past the last step repeat it; none lies under a condition, and the loop is left
@@ -396,55 +434,64 @@ __global__ __launch_bounds__(kThreads) void k_attend(const Args a) {
       turn(std::integral_constant<int, 2>{}, step + 2 * kWaves);
     }
   }
-  sum = group_sum(sum);
+#pragma unroll
+  for (int t = 0; t < QT; ++t) sum[t] = group_sum(sum[t]);
 
-  // Join the wavefronts: the upper half into the lower, and so on.
-  __syncthreads();  // nothing reads or loads the steps' rooms any more
+  // Join the wavefronts, a tile of rows at a time: the upper half into the lower, and so on.
   f32x4 (*room)[C][64] = reinterpret_cast<f32x4 (*)[C][64]>(step_room<D, 0>());
   static_assert(kWaves / 2 * C * 1024 <= kWaves * 32 * D, "joined outputs outgrow a room");
 #pragma unroll
-  for (int half = kWaves / 2; half; half /= 2) {
-    if (wave >= half && wave < 2 * half) {
-      if (g == 0) stats[wave][i16] = make_float2(top, sum);
+  for (int t = 0; t < QT; ++t) {
 #pragma unroll
-      for (int j = 0; j < C; ++j) room[wave - half][j][lane] = o[j];
-    }
-    __syncthreads();
-    if (wave < half) {
-      const float2 other = stats[wave + half][i16];
-      const float raised = fmaxf(top, other.x), base = reference_of(raised);
-      const float mine = exp2_of(top - base), theirs = exp2_of(other.x - base);
-      top = raised;
-      sum = fma_rn(sum, mine, other.y * theirs);
+    for (int half = kWaves / 2; half; half /= 2) {
+      __syncthreads();  // nothing reads what is written next any more
+      if (wave >= half && wave < 2 * half) {
+        if (g == 0) stats[wave][i16] = make_float2(top[t], sum[t]);
 #pragma unroll
-      for (int j = 0; j < C; ++j) o[j] = o[j] * mine + room[wave][j][lane] * theirs;
+        for (int j = 0; j < C; ++j) room[wave - half][j][lane] = o[t][j];
+      }
+      __syncthreads();
+      if (wave < half) {
+        const float2 other = stats[wave + half][i16];
+        const float raised = fmaxf(top[t], other.x), base = reference_of(raised);
+        const float mine = exp2_of(top[t] - base), theirs = exp2_of(other.x - base);
+        top[t] = raised;
+        sum[t] = fma_rn(sum[t], mine, other.y * theirs);
+#pragma unroll
+        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * mine + room[wave][j][lane] * theirs;
+      }
     }
-    __syncthreads();
   }
-  if (wave || i16 >= count) return;
-  // The lane's features (4 g + r) C + j of its row.
-  if (a.splits == 1) {
-    T* out = static_cast<T*>(a.out) + query_offset(a, row, kvh);
-    const float by = sight.end ? 1.0f : 0.0f;
+  if (wave) return;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    if (16u * t + i16 >= count) continue;
+    // The lane's features (4 g + r) C + j of its row.
+    if (a.splits == 1) {
+      T* out = static_cast<T*>(a.out) + query_offset(a, row_of(t), kvh);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < C; j += 4) {
+          const uint32_t f = (4 * g + r) * C + j;
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = sight[t].end ? o[t][j + e][r] / sum[t] : 0.0f;
+          if (f < a.width) store_four(out + f, v, a.width - f, a.whole_out);
+        }
+      continue;
+    }
+    const uint64_t place = (static_cast<uint64_t>(range) * a.kv_heads + kvh) * a.all_rows + row_of(t);
+    if (g == 0) a.part[place] = make_float2(top[t], sum[t]);
+    float* to = a.sums + place * a.pitch;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int j = 0; j < C; ++j) {
+      for (int j = 0; j < C; j += 4) {
         const uint32_t f = (4 * g + r) * C + j;
-        if (f < a.width) store_elem(out, f, by == 0.0f ? 0.0f : o[j][r] / sum);
+        if (f < a.pitch) *reinterpret_cast<f32x4*>(to + f) = f32x4{o[t][j][r], o[t][j + 1][r], o[t][j + 2][r], o[t][j + 3][r]};
       }
-    return;
   }
-  const uint64_t place = (static_cast<uint64_t>(range) * a.kv_heads + kvh) * a.all_rows + row;
-  if (g == 0) a.part[place] = make_float2(top, sum);
-  float* to = a.sums + place * a.pitch;
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-#pragma unroll
-    for (int j = 0; j < C; j += 4) {
-      const uint32_t f = (4 * g + r) * C + j;
-      if (f < a.pitch) *reinterpret_cast<f32x4*>(to + f) = f32x4{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
-    }
 }
 
 // Joins the ranges of one row, W wavefronts a row.  D / 4 lanes hold a row of a range,
@@ -458,7 +505,7 @@ __global__ __launch_bounds__(kThreads) void k_join(const Args a) {
   const uint32_t tasks = a.kv_heads * a.all_rows, task = blockIdx.x * kTasks + wave / W;
   if (task >= tasks) return;  // wavefronts of one row end together
   const uint32_t row = task % a.all_rows, kvh = task / a.all_rows;
-  const uint32_t in_seq = row % a.seq_rows, tile = in_seq / 16, n = length_of(a, row / a.seq_rows);
+  const uint32_t in_seq = row % a.seq_rows, tile0 = in_seq / a.tile_rows * a.tile_rows, n = length_of(a, row / a.seq_rows);
   const uint32_t f = lane % kLanes * 4, first = wave % W * (64 / kLanes) + lane / kLanes;
   const float* sums = a.sums + (f < a.pitch ? f : 0);
   f32x4 ahead[kAhead];
@@ -466,7 +513,7 @@ __global__ __launch_bounds__(kThreads) void k_join(const Args a) {
   for (uint32_t m = 0; m < kAhead; ++m)
     ahead[m] = *reinterpret_cast<const f32x4*>(sums + (static_cast<uint64_t>(min(m * kAtOnce + first, a.splits - 1)) * tasks + task) * a.pitch);
   const Sight sight = sight_of(a, n, in_seq / a.group);
-  const Steps steps(a, sight_of(a, n, tile * 16 / a.group), sight_of(a, n, min(tile * 16 + 15, a.seq_rows - 1) / a.group));
+  const Steps steps(a, sight_of(a, n, tile0 / a.group), sight_of(a, n, (min(tile0 + a.tile_rows, a.seq_rows) - 1) / a.group));
   const uint32_t each = range_steps(steps.count, a.splits), ranges = steps.count ? (steps.count + each - 1) / each : 0;
   auto part = [&](uint32_t r) { return a.part[static_cast<uint64_t>(r) * tasks + task]; };
   const float2 mine = lane < ranges ? part(lane) : make_float2(-INFINITY, 0.0f);
@@ -503,15 +550,15 @@ __global__ __launch_bounds__(kThreads) void k_join(const Args a) {
     for (int w = 1; w < W; ++w) acc = acc + room[w][lane];
   }
   if (lane >= kLanes) return;
-  T* out = static_cast<T*>(a.out) + query_offset(a, row, kvh);
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (f + e < a.width) store_elem(out, f + e, sight.end ? acc[e] / sum : 0.0f);
+  for (int e = 0; e < 4; ++e) acc[e] = sight.end ? acc[e] / sum : 0.0f;
+  if (f < a.width) store_four(static_cast<T*>(a.out) + query_offset(a, row, kvh) + f, acc, a.width - f, a.whole_out);
 }
 
 // ------------------------------------------------------------------- the host
 constexpr uint64_t kMostBlocks = (1u << 23) - 8;
 constexpr uint32_t kFewRanges = 8;
+constexpr uint64_t kMostRange = 8192;  // keys
 
 uint64_t times(uint64_t x, uint64_t y, uint64_t most, const char* what) {
   require(y == 0 || x <= most / y, what, DL_LENGTH_ERROR);
@@ -525,7 +572,7 @@ struct Layout {
   uint64_t bytes() const { return part_bytes + sums_bytes; }
 };
 
-Layout layout_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks) {
+Layout layout_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks, bool bf16) {
   batch::check_shape(shape);
   require(shape->width <= 256, "head width above 256", DL_LENGTH_ERROR);
   Layout l;
@@ -545,14 +592,19 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks) {
   a.seq_rows = static_cast<uint32_t>(times(a.rows, a.group, 1u << 30, kRows));
   a.all_rows = static_cast<uint32_t>(times(a.seq_rows, a.batch, 1u << 30, kRows));
   times(a.all_rows, a.kv_heads, 1u << 23, kRows);  // workgroups of the join
-  a.tiles = static_cast<uint32_t>(ceil_div(a.seq_rows, 16));
+  // Two tiles a wavefront convert the keys and values once for both.  BF16, 512 rows of
+  // 32 heads over 4096 keys: 62 us, one tile 89; 1000 rows of them, 511 keys in sight each:
+  // 44 and 56; 64 rows a KV head, 4 sequences: 23 and 22.  FP32, with three products for
+  // one: 140 and 129.  Of 256 features two tiles do not fit the registers.
+  a.tile_rows = bf16 && a.width <= 128 && a.seq_rows > 64 ? 32 : 16;
+  a.tiles = static_cast<uint32_t>(ceil_div(a.seq_rows, a.tile_rows));
   a.pitch = (a.width + 3) / 4 * 4;
   // Most steps that a row tile can see, and ranges for two workgroups a compute unit.
   uint64_t keys = a.capacity;
-  if (a.window) keys = std::min<uint64_t>(keys, uint64_t{a.window} + a.sinks + 16 + 3 * kKeys);
+  if (a.window) keys = std::min<uint64_t>(keys, uint64_t{a.window} + a.sinks + a.tile_rows + 3 * kKeys);
   const uint64_t rounds = ceil_div(keys, kKeys * kWaves);
   const uint64_t tasks = times(times(a.batch, a.kv_heads, kMostBlocks, "too many workgroups"), a.tiles, kMostBlocks, "too many workgroups");
-  a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(ceil_div(rounds, 2), ceil_div(1024, tasks))));
+  a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(ceil_div(rounds, 2), std::max(ceil_div(512, tasks), keys / kMostRange))));
   const uint64_t groups = times(uint64_t{a.batch} * a.kv_heads, a.splits, kMostBlocks, "too many workgroups");
   l.blocks = static_cast<uint32_t>(times(ceil_div(groups, 8) * 8, a.tiles, kMostBlocks, "too many workgroups"));
   if (a.splits > 1) {
@@ -563,12 +615,26 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks) {
   return l;
 }
 
+// One size for either storage type, whose tiles and so ranges differ.
+uint64_t bytes_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks) {
+  return std::max(layout_of(shape, window, sinks, true).bytes(), layout_of(shape, window, sinks, false).bytes());
+}
+
 template <class T, int D>
 void launch(hipStream_t s, const Layout& l, bool pieces) {
-  if (pieces)
-    k_attend<T, D, true><<<l.blocks, kThreads, 0, s>>>(l.args);
-  else
-    k_attend<T, D, false><<<l.blocks, kThreads, 0, s>>>(l.args);
+  auto attend = [&](auto tiles) {
+    constexpr int QT = decltype(tiles)::value;
+    if (pieces)
+      k_attend<T, D, true, QT><<<l.blocks, kThreads, 0, s>>>(l.args);
+    else
+      k_attend<T, D, false, QT><<<l.blocks, kThreads, 0, s>>>(l.args);
+  };
+  bool one = true;
+  if constexpr (sizeof(T) == 2 && D < 256) one = l.args.tile_rows == 16;
+  if (one)
+    attend(std::integral_constant<int, 1>{});
+  else if constexpr (sizeof(T) == 2 && D < 256)
+    attend(std::integral_constant<int, 2>{});
   // A workgroup per row where there are many ranges, else a wavefront.
   const uint64_t tasks = uint64_t{l.args.kv_heads} * l.args.all_rows;
   if (l.args.splits > kFewRanges)
@@ -598,7 +664,7 @@ extern "C" {
 int dl_attention_fp4_bytes(const dl_batch_shape* shape, uint64_t window, uint64_t sinks, uint64_t* bytes) {
   return guard([&] {
     require(bytes != nullptr, "null output");
-    *bytes = dl::fp4::layout_of(shape, window, sinks).bytes();
+    *bytes = dl::fp4::bytes_of(shape, window, sinks);
   });
 }
 
@@ -608,14 +674,15 @@ int dl_attention_fp4(dl_queue* queue, int dtype, const dl_batch_shape* shape, co
   return guard([&] {
     using namespace dl::fp4;
     require(dtype == DL_BF16 || dtype == DL_F32, "unsupported storage type");
-    Layout l = layout_of(shape, window, sinks);
+    Layout l = layout_of(shape, window, sinks, dtype == DL_BF16);
+    const uint64_t bytes = bytes_of(shape, window, sinks);
     require(cache != nullptr, "null cache");
     require(query && cache->key_codes && cache->key_scales && cache->value_codes && cache->value_scales && lengths && output && scale,
             "null operand");
     auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     require(aligned(cache->key_codes) && aligned(cache->value_codes), "codes not 16-byte aligned");
-    require(l.bytes() == 0 || (workspace != nullptr && aligned(workspace)), "workspace null or not 16-byte aligned");
-    require(workspace_bytes >= l.bytes(), "workspace too small", DL_LENGTH_ERROR);
+    require(bytes == 0 || (workspace != nullptr && aligned(workspace)), "workspace null or not 16-byte aligned");
+    require(workspace_bytes >= bytes, "workspace too small", DL_LENGTH_ERROR);
     dl::enter(queue);
     Args& a = l.args;
     a.query = query;
@@ -626,6 +693,7 @@ int dl_attention_fp4(dl_queue* queue, int dtype, const dl_batch_shape* shape, co
     a.lengths = lengths;
     a.scale = scale;
     a.out = output;
+    a.whole_out = shape->width % 4 == 0 && reinterpret_cast<uintptr_t>(output) % (dtype == DL_BF16 ? 8 : 16) == 0;
     a.part = static_cast<float2*>(workspace);
     a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + l.part_bytes);
     const bool pieces = (shape->width * (dtype == DL_BF16 ? 2 : 4)) % 16 == 0 && aligned(query);
