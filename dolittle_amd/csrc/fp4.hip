@@ -660,18 +660,69 @@ __device__ __forceinline__ void advance(const AppendArgs& a, uint64_t b) {
   a.positions_out[b] = first + a.rows;
 }
 
+// Four features of a row at whole alignment.
+template <class T>
+__device__ __forceinline__ f32x4 load_four(const T* from) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const f32x4*>(from);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(from);
+    return f32x4{dl_bf16_lo(v.x), dl_bf16_hi(v.x), dl_bf16_lo(v.y), dl_bf16_hi(v.y)};
+  }
+}
+
 // One workgroup per new row.  Cosines and sines of a row are computed once, in 64
 // bits from the catalog's FP32 angle; rotated keys go from FP32 to 4 bits in one
 // rounding.  32 lanes take a head, eight features each, and four of them a group.
-template <class T>
+// What bounds it for few rows is one wait for memory and the 64-bit angles, so the
+// rows are asked for before the angles are computed.  kFours: halves are of
+// whole fours, all rows at their alignment.
+template <class T, bool kFours>
 __global__ __launch_bounds__(kAppendThreads) void k_append(const AppendArgs a, bool advance_here) {
-  __shared__ float cosine[kMostWidth / 2], sine[kMostWidth / 2];
+  __shared__ __align__(16) float cosine[kMostWidth / 2], sine[kMostWidth / 2];
+  constexpr uint32_t kEach = kFours ? 4 : 1, kAhead = kFours ? 2 : 1;  // features of a query piece, pieces asked for early
+  using Each = std::conditional_t<kFours, f32x4, float>;
   const uint64_t b = blockIdx.y;
   const uint32_t half = a.width / 2, groups = (a.width + kGroup - 1) / kGroup;
+  const uint32_t in_half = half / kEach, pieces = a.q_heads * in_half, f0 = threadIdx.x % 32 * 8;
+  auto load = [](const T* from) __attribute__((always_inline)) {
+    if constexpr (kFours)
+      return load_four(from);
+    else
+      return load_elem(from, 0);
+  };
   const uint64_t n = a.lengths[b], first = a.positions[b];
   for (uint64_t i = blockIdx.x; i < a.rows; i += gridDim.x) {
     const uint64_t position = first + i, slot = n + i, row = b * a.rows + i;
     const bool fits = n < a.capacity && i < a.capacity - n;
+    const T* query = static_cast<const T*>(a.query) + row * a.q_heads * a.width;
+    T* query_out = static_cast<T*>(a.query_out) + row * a.q_heads * a.width;
+    Each lower[kAhead], upper[kAhead];
+#pragma unroll
+    for (uint32_t x = 0; x < kAhead; ++x) {
+      const uint32_t p = min(threadIdx.x + x * kAppendThreads, pieces - 1), at = p / in_half * a.width + p % in_half * kEach;
+      lower[x] = load(query + at);
+      upper[x] = load(query + at + half);
+    }
+    // Of a head the lane's features, those half a row away, and its values.
+    float k[8], other[8], v[8];
+    auto ask = [&](uint32_t h) __attribute__((always_inline)) {
+      const uint64_t from = (row * a.kv_heads + min(h, a.kv_heads - 1)) * a.width;
+      const T* key = static_cast<const T*>(a.key) + from;
+      const T* value = static_cast<const T*>(a.value) + from;
+#pragma unroll
+      for (uint32_t e = 0; e < 8; e += kEach) {
+        const uint32_t f = f0 + e < a.width ? f0 + e : 0, o = f < half ? f + half : f - half;
+        const Each at = load(key + f), away = load(key + o), val = load(value + f);
+        if constexpr (kFours) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) k[e + c] = at[c], other[e + c] = away[c], v[e + c] = val[c];
+        } else {
+          k[e] = at, other[e] = away, v[e] = val;
+        }
+      }
+    };
+    ask(threadIdx.x / 32);
     for (uint32_t f = threadIdx.x; f < half; f += kAppendThreads) {
       const float exponent = static_cast<float>(2 * f) / static_cast<float>(a.width);
       const float frequency = static_cast<float>(1.0 / dl_pow_pos(a.theta, static_cast<double>(exponent)));
@@ -682,39 +733,40 @@ __global__ __launch_bounds__(kAppendThreads) void k_append(const AppendArgs a, b
       sine[f] = static_cast<float>(s);
     }
     __syncthreads();
-    const T* query = static_cast<const T*>(a.query) + row * a.q_heads * a.width;
-    T* query_out = static_cast<T*>(a.query_out) + row * a.q_heads * a.width;
-    for (uint32_t p = threadIdx.x; p < a.q_heads * half; p += kAppendThreads) {
-      const uint32_t at = p / half * a.width, f = p % half;
-      const float u = load_elem(query, at + f), v = load_elem(query, at + half + f), c = cosine[f], s = sine[f];
-      store_elem(query_out, at + f, u * c - v * s);
-      store_elem(query_out, at + half + f, v * c + u * s);
+    auto turn = [&](uint32_t p, const Each& u, const Each& v) __attribute__((always_inline)) {
+      const uint32_t f = p % in_half * kEach, at = p / in_half * a.width + f;
+      if constexpr (kFours) {
+        const f32x4 c = *reinterpret_cast<const f32x4*>(cosine + f), s = *reinterpret_cast<const f32x4*>(sine + f);
+        store_four(query_out + at, u * c - v * s, 4, true);
+        store_four(query_out + at + half, v * c + u * s, 4, true);
+      } else {
+        store_elem(query_out, at, u * cosine[f] - v * sine[f]);
+        store_elem(query_out, at + half, v * cosine[f] + u * sine[f]);
+      }
+    };
+#pragma unroll
+    for (uint32_t x = 0; x < kAhead; ++x)
+      if (threadIdx.x + x * kAppendThreads < pieces) turn(threadIdx.x + x * kAppendThreads, lower[x], upper[x]);
+    for (uint32_t p = threadIdx.x + kAhead * kAppendThreads; p < pieces; p += kAppendThreads) {
+      const uint32_t at = p / in_half * a.width + p % in_half * kEach;
+      turn(p, load(query + at), load(query + at + half));
     }
     if (fits) {
-      const uint32_t f0 = threadIdx.x % 32 * 8;
       // Both halves of a wavefront run every pass: shuffles need their lanes.
       for (uint32_t h0 = 0; h0 < a.kv_heads; h0 += kAppendThreads / 32) {
         const uint32_t h = h0 + threadIdx.x / 32;
-        const bool real = h < a.kv_heads;
-        const uint64_t from = (row * a.kv_heads + (real ? h : 0)) * a.width;
-        const uint64_t to = ((b * a.kv_heads + h) * a.capacity + slot) * groups;
-        const T* key = static_cast<const T*>(a.key) + from;
-        const T* value = static_cast<const T*>(a.value) + from;
-        float k[8], v[8];
+        if (h0) ask(h);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t f = f0 + e;
-          k[e] = v[e] = 0.0f;
-          if (f < a.width) {
-            const float x = load_elem(key, f);
-            k[e] = f < half ? x * cosine[f] - load_elem(key, f + half) * sine[f]
-                            : x * cosine[f - half] + load_elem(key, f - half) * sine[f - half];
-            v[e] = load_elem(value, f);
-          }
+          if (f >= a.width)
+            k[e] = v[e] = 0.0f;
+          else
+            k[e] = f < half ? k[e] * cosine[f] - other[e] * sine[f] : k[e] * cosine[f - half] + other[e] * sine[f - half];
         }
         const uint32_t k_byte = scale_byte(group_largest(largest_of(k))), v_byte = scale_byte(group_largest(largest_of(v)));
-        if (real && f0 < groups * kGroup) {
-          const uint64_t at = to * 4 + f0 / 8;
+        if (h < a.kv_heads && f0 < groups * kGroup) {
+          const uint64_t at = ((b * a.kv_heads + h) * a.capacity + slot) * groups * 4 + f0 / 8;
           static_cast<uint32_t*>(a.cache.key_codes)[at] = to_codes(k, k_byte);
           static_cast<uint32_t*>(a.cache.value_codes)[at] = to_codes(v, v_byte);
           if (f0 % kGroup == 0) {
@@ -859,10 +911,11 @@ int dl_cache_append_fp4(dl_queue* queue, int dtype, const dl_batch_shape* shape,
     // one, which may be the same word; of several any may still have to.
     const bool apart = lengths != lengths_out && positions != positions_out && lengths != positions_out && positions != lengths_out;
     const bool advance_here = grid.x == 1 || apart;
-    if (dtype == DL_BF16)
-      k_append<uint16_t><<<grid, kAppendThreads, 0, queue->stream>>>(a, advance_here);
-    else
-      k_append<float><<<grid, kAppendThreads, 0, queue->stream>>>(a, advance_here);
+    const uint64_t four = dtype == DL_BF16 ? 8 : 16;
+    const bool fours = shape->width % 8 == 0 && aligned(query, four) && aligned(key, four) && aligned(value, four) && aligned(query_out, four);
+    with_type(dtype, fours, [&](auto type, auto whole) {
+      k_append<decltype(type), decltype(whole)::value><<<grid, kAppendThreads, 0, queue->stream>>>(a, advance_here);
+    });
     if (!advance_here)
       k_advance<<<static_cast<unsigned>(dl::ceil_div(shape->batch, 64)), 64, 0, queue->stream>>>(a, shape->batch);
     dl::check_launch(queue, "cache_append_fp4");
