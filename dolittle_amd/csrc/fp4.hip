@@ -611,9 +611,9 @@ void launch_project(hipStream_t s, const ProjectArgs& a) {
     return;
   }
   const uint64_t row_tiles = ceil_div(a.rows, columns_of<T>);
-  require(row_tiles <= 65535, "too many rows", DL_LENGTH_ERROR);
 #define I(n) std::integral_constant<int, n>{}
   if (a.groups > 384) {
+    require(a.out_w <= (1u << 26), "too many workgroups", DL_LENGTH_ERROR);
     const dim3 grid(static_cast<unsigned>(ceil_div(a.out_w, 16)), static_cast<unsigned>(row_tiles));
     k_project_long<T, kPieces><<<grid, kProjectWaves * 64, 0, s>>>(a);
     return;

@@ -330,8 +330,8 @@ int dl_fp4_quantize(dl_queue* queue, int dtype, const void* input, void* codes, 
 int dl_fp4_values(dl_queue* queue, int dtype, const void* codes, const void* scales, void* output, uint64_t rows,
                   uint64_t width);
 /* dl_projection with 4-bit weights: Y[R,O] = X[R,I] W[O,I]^T, one rounding of the
- * FP32 sum.  Fast for one to 16 rows, which read the weights once; a NaN group
- * makes its output NaN. */
+ * FP32 sum.  Up to 32 rows (FP32 20) read the weights once per 16 (5) of them, more
+ * convert them once per 32 or 64; a NaN group makes its output NaN. */
 int dl_projection_fp4(dl_queue* queue, int dtype, const void* input, const void* codes, const void* scales,
                       void* output, uint64_t rows, uint64_t input_width, uint64_t output_width,
                       const uint64_t* output_position);

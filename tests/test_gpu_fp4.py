@@ -178,6 +178,27 @@ def test_projection_special_values(oracle, device, queue, dtype, rows):
     close(got[plain], want[plain], bound[plain])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,inputs,outputs,shift,position", [(40, 12500, 70, 0, None), (5, 8330, 50, 1, None), (3, 12288, 20, 1, 2),
+                                                                (70, 416, 130, 1, 4), (21, 4096, 40, 0, 1), (150, 1056, 1100, 0, None),
+                                                                (33, 1, 1, 0, None), (4, 12320, 33, 1, None)])
+def test_projection_other_forms(oracle, device, queue, dtype, rows, inputs, outputs, shift, position):
+    """Long rows in many, scales that are no whole words in every form, one input, both sides of the rules."""
+    rng = np.random.default_rng(rows + inputs)
+    x = stored(oracle, rng.standard_normal((rows, inputs)), dtype)
+    codes, scales = packed_random(rng, (outputs, inputs), inputs ** -0.5)
+    want, bound = ref.projection(value_of(x), ref.values(codes, scales, inputs), dtype)
+    close(project(device, queue, dtype, x, codes, scales, rows, inputs, outputs, shift, position), want, bound)
+
+
+def test_projection_refuses_too_many_outputs(device, queue):
+    room = device.allocate(1 << 16)
+    at = room.ptr()
+    for rows, inputs, outputs in ((1, 16384, 1 << 30), (1 << 30, 64, 1 << 30), ((1 << 30) + 1, 64, 1), (1, 64, (1 << 30) + 1)):
+        with pytest.raises(_lib.DolittleError, match="too (large|many)"):
+            _lib.call("dl_projection_fp4", queue.handle, 1, at, at, at, at, rows, inputs, outputs, None)
+
+
 def test_projection_same_bits(oracle, device, queue):
     rng = np.random.default_rng(2)
     x = stored(oracle, rng.standard_normal((4, 4096)), "bf16")
