@@ -11,7 +11,10 @@
 // times the heads of the group) and a range of the steps of 32 keys that any of them
 // sees; its wavefronts take every fourth step, whose codes come through LDS rooms of
 // their own, two steps ahead.  Ranges leave their maximum, sum and unnormalised
-// output, which k_join joins; a single range writes the output itself.
+// output, which k_join joins; a single range writes the output itself.  Of few rows the
+// caches' stream is the bound: 64 sequences of up to 32,768 keys, 8 KV heads of 128
+// features, 292 us, 5.2 TB/s; of many the conversions and exponentials beside the
+// products: 512 rows of 32 heads over 4096 keys 59 us, 540 TFLOP/s, FP32 123.
 //
 // Operands.  A lane takes D / 4 neighbouring features of a key's codes, one to two
 // groups or half of one, and converts them to the first operands of the products K
@@ -171,18 +174,19 @@ struct Tile {
   static constexpr int kValueWords = C < 8 ? 1 : C / 8;       // D = 64: four codes, the lower half of a word
 };
 
-// A step's codes of one wavefront: 32 keys, then their values, D / 2 bytes each.
-// Objects apart, so that the compiler sees no use of loads in flight.
+// A step's codes of one wavefront: 32 keys, then their values, D / 2 bytes each, and
+// with kWords their scales, D / 32 bytes each.  Objects apart, so that the compiler sees
+// no use of loads in flight.
 constexpr int kRing = 3;
-template <int D, int kSlot>
+template <int D, int kSlot, bool kWords>
 __device__ __forceinline__ uint8_t* step_room() {
-  __shared__ __align__(1024) uint8_t room[kWaves * 32 * D];
+  __shared__ __align__(1024) uint8_t room[kWaves * (32 * D + (kWords ? 2 * D : 0))];
   return room;
 }
 
 // Of two tiles of rows a wavefront holds twice the queries and outputs: left to itself
 // the compiler takes 300 registers, one workgroup a unit, 91 us where this takes 62.
-template <class T, int D, bool kPieces, int QT>
+template <class T, int D, bool kPieces, bool kWords, int QT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) void k_attend(const Args a) {
   using S = Tile<T, D>;
   constexpr int C = S::C, kParts = S::kParts;
@@ -226,7 +230,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
   // bytes to registers as far ahead.  Features past the row's last group repeat it: the
   // query has zeros there, and such features of the output are not stored.  Piece p of a
   // key's codes lies at p ^ key / 8, so that the keys of an operand lie in distinct banks.
+  // Whole rows of scale words go through LDS too, 1 load (D = 256: 2) for 10 (12): 512 rows
+  // over 4096 keys 59.5 us for 61.6, 8 sequences of 4607 keys 18.0 for 18.5.
   constexpr uint32_t P = D / 32, kRowBytes = D / 2, kHalf = 16 * D;  // pieces of a key; bytes of 32
+  constexpr uint32_t kRoom = 2 * kHalf + (kWords ? 2 * D : 0), kWordRow = kWords ? D / 128 : 1;
   const uint32_t value_group = min(i16 * C / kGroup, a.groups - 1);
   struct Scales {
     uint32_t key[2][S::kKeyScales], value[8];
@@ -238,13 +245,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
     const uint8_t* vc = value_codes + static_cast<uint64_t>(at) * row_bytes;
     const uint8_t* ks = key_scales + static_cast<uint64_t>(at) * a.groups;
     const uint8_t* vs = value_scales + static_cast<uint64_t>(at) * a.groups;
-    uint8_t* mine = room + wave * (2 * kHalf);
+    uint8_t* mine = room + wave * kRoom;
 #pragma unroll
     for (uint32_t x = 0; x < kHalf / 1024; ++x) {
       const uint32_t slot = x * 64 + lane, key = slot / P, piece = min(slot % P ^ key / 8 % P, a.groups - 1);
       const uint32_t from = min(key, last) * row_bytes + piece * kGroupBytes;
       __builtin_amdgcn_global_load_lds((const global_ptr*)(kc + from), (lds_ptr*)(mine + x * 1024), 16, 0, 0);
       __builtin_amdgcn_global_load_lds((const global_ptr*)(vc + from), (lds_ptr*)(mine + kHalf + x * 1024), 16, 0, 0);
+    }
+    if constexpr (kWords) {
+#pragma unroll
+      for (uint32_t x = 0; x < kWordRow; ++x) {
+        const uint32_t word = x * 64 + lane, in_half = word % (32 * kWordRow);
+        const uint8_t* of = word < 32 * kWordRow ? ks : vs;
+        __builtin_amdgcn_global_load_lds((const global_ptr*)(of + min(in_half / kWordRow, last) * P + in_half % kWordRow * 4),
+                                         (lds_ptr*)(mine + 2 * kHalf + x * 256), 4, 0, 0);
+      }
+      return;
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -255,7 +272,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
 #pragma unroll
     for (int e = 0; e < 8; ++e) to.value[e] = vs[min(8 * g + e, last) * a.groups + value_group];
   };
-  constexpr int kLoads = 2 * kHalf / 1024 + 2 * S::kKeyScales + 8;
+  constexpr int kLoads = 2 * kHalf / 1024 + (kWords ? kWordRow : 2 * S::kKeyScales + 8);
 
   f32x4 o[QT][C];
   float top[QT], from[QT], most_sum[QT], sum[QT];
@@ -269,7 +286,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
   }
 
   auto work = [&](const uint8_t* room, const Scales& by, uint32_t at) __attribute__((always_inline)) {
-    const uint8_t* keys = room + wave * (2 * kHalf);
+    const uint8_t* keys = room + wave * kRoom;
     // No branch, which the && and || would be, lies between products and their use.
     const bool masked = (at + kKeys > least.end) | ((a.window != 0) & (at < most.low) & (at + kKeys > a.sinks));
     // Scores of the lane's rows and the keys at + 8 g + 4 u + r.
@@ -294,7 +311,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
       for (int t = 0; t < QT; ++t) p[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < S::kSteps; ++s) {
-        const u32x4 k = to_bf16(words[s], scale_of(by.key[u][s * S::kKeyScales / S::kSteps]));
+        const int h = s * S::kKeyScales / S::kSteps;
+        const u32x4 k = to_bf16(words[s], scale_of(kWords ? keys[2 * kHalf + key * P + g * (D / 4) / kGroup + h] : by.key[u][h]));
 #pragma unroll
         for (int i = 0; i < kParts; ++i)
 #pragma unroll
@@ -305,7 +323,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
     uint32_t words[8][S::kValueWords], bytes[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      bytes[e] = by.value[e];
+      bytes[e] = kWords ? keys[2 * kHalf + D + (8 * g + e) * P + value_group] : by.value[e];
       const uint32_t byte = i16 * (C / 2);  // of the key's codes
       const uint8_t* from = keys + kHalf + (8 * g + e) * kRowBytes + (byte / 16 ^ g % P) * 16 + byte % 16;
       if constexpr (C == 4) {
@@ -418,15 +436,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
     constexpr int kSlot = decltype(slot)::value, kNext = (kSlot + kRing - 1) % kRing;
     __builtin_amdgcn_s_waitcnt(lds_wait((kRing - 2) * kLoads));  // this step's codes; the room loaded next is read
     asm volatile("" ::: "memory");
-    load(step_room<D, kNext>(), ring[kNext], steps.key(min(step + (kRing - 1) * kWaves, end - 1)));
+    load(step_room<D, kNext, kWords>(), ring[kNext], steps.key(min(step + (kRing - 1) * kWaves, end - 1)));
     __builtin_amdgcn_sched_barrier(0);
-    if (step < end) work(step_room<D, kSlot>(), ring[kSlot], steps.key(step));
+    if (step < end) work(step_room<D, kSlot, kWords>(), ring[kSlot], steps.key(step));
   };
   uint32_t step = begin + wave;
   if (step < end) {
-    load(step_room<D, 0>(), ring[0], steps.key(step));
+    load(step_room<D, 0, kWords>(), ring[0], steps.key(step));
     __builtin_amdgcn_sched_barrier(0);
-    load(step_room<D, 1>(), ring[1], steps.key(min(step + kWaves, end - 1)));
+    load(step_room<D, 1, kWords>(), ring[1], steps.key(min(step + kWaves, end - 1)));
     __builtin_amdgcn_sched_barrier(0);
     for (; step < end; step += kRing * kWaves) {
       turn(std::integral_constant<int, 0>{}, step);
@@ -438,7 +456,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
   for (int t = 0; t < QT; ++t) sum[t] = group_sum(sum[t]);
 
   // Join the wavefronts, a tile of rows at a time: the upper half into the lower, and so on.
-  f32x4 (*room)[C][64] = reinterpret_cast<f32x4 (*)[C][64]>(step_room<D, 0>());
+  f32x4 (*room)[C][64] = reinterpret_cast<f32x4 (*)[C][64]>(step_room<D, 0, kWords>());
   static_assert(kWaves / 2 * C * 1024 <= kWaves * 32 * D, "joined outputs outgrow a room");
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -621,13 +639,16 @@ uint64_t bytes_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks) 
 }
 
 template <class T, int D>
-void launch(hipStream_t s, const Layout& l, bool pieces) {
+void launch(hipStream_t s, const Layout& l, bool pieces, bool words) {
   auto attend = [&](auto tiles) {
     constexpr int QT = decltype(tiles)::value;
+    if constexpr (D >= 128) {
+      if (pieces && words) return k_attend<T, D, true, true, QT><<<l.blocks, kThreads, 0, s>>>(l.args);
+    }
     if (pieces)
-      k_attend<T, D, true, QT><<<l.blocks, kThreads, 0, s>>>(l.args);
+      k_attend<T, D, true, false, QT><<<l.blocks, kThreads, 0, s>>>(l.args);
     else
-      k_attend<T, D, false, QT><<<l.blocks, kThreads, 0, s>>>(l.args);
+      k_attend<T, D, false, false, QT><<<l.blocks, kThreads, 0, s>>>(l.args);
   };
   bool one = true;
   if constexpr (sizeof(T) == 2 && D < 256) one = l.args.tile_rows == 16;
@@ -645,12 +666,16 @@ void launch(hipStream_t s, const Layout& l, bool pieces) {
 
 template <class T>
 void launch_width(hipStream_t s, const Layout& l, bool pieces) {
-  if (l.args.width <= 64)
-    launch<T, 64>(s, l, pieces);
-  else if (l.args.width <= 128)
-    launch<T, 128>(s, l, pieces);
+  const Args& a = l.args;
+  // All groups of the tile's width, in words: whole rows.
+  const bool words = a.groups == (a.width <= 128 ? 4 : 8) && reinterpret_cast<uintptr_t>(a.key_scales) % 4 == 0 &&
+                     reinterpret_cast<uintptr_t>(a.value_scales) % 4 == 0;
+  if (a.width <= 64)
+    launch<T, 64>(s, l, pieces, false);
+  else if (a.width <= 128)
+    launch<T, 128>(s, l, pieces, words);
   else
-    launch<T, 256>(s, l, pieces);
+    launch<T, 256>(s, l, pieces, words);
 }
 
 }  // namespace

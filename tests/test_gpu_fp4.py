@@ -284,6 +284,14 @@ def test_attention_chunks(oracle, device, queue, dtype, rows, capacity, heads, w
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("heads", [(4, 2, 104), (4, 1, 232), (2, 2, 128), (3, 1, 256)])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_attention_rows_of_scale_words(oracle, device, queue, dtype, heads, rows):
+    """Rows whose scales are whole words but whose last group is not full; lengths inside a step."""
+    Problem(oracle, dtype, 3, rows, 333, heads, [333, 97, 71], seed=3).check(device, queue)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("window", [0, 3000])
 def test_attention_long(oracle, device, queue, dtype, window):
     """Many ranges of one long cache, joined."""
