@@ -144,29 +144,35 @@ __device__ __forceinline__ void query_operands(const T* row, uint32_t at, uint32
   }
 }
 
-// Eight exponentials as product operands: rounded to BF16 for BF16 storage (at most
-// 2^-8 of the value, as BF16 operands need), exact in three parts for FP32.
-template <int kParts>
-__device__ __forceinline__ void share_operands(const f32x4 (&p)[2], u32x4 (&b)[kParts]) {
-  if constexpr (kParts == 3) {
-    float x[8];
+// Eight exponentials as product operands: exact in three parts for FP32 storage, for
+// BF16 in two, what the first leaves rounded again: at most 2^-16 of the value.  One part
+// alone, 2^-8, is as far off as the output's own rounding and more where values cancel.
+template <int kShares>
+__device__ __forceinline__ void share_operands(const f32x4 (&p)[2], u32x4 (&b)[kShares]) {
+  float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = p[e / 4][e % 4];
+  for (int e = 0; e < 8; ++e) x[e] = p[e / 4][e % 4];
+  if constexpr (kShares == 3) {
     const Parts s = split(x);
 #pragma unroll
     for (int i = 0; i < 3; ++i) b[i] = s.part[i];
   } else {
-    bf16x8 v;
+    bf16x8 high, low;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = static_cast<__bf16>(p[e / 4][e % 4]);
-    b[0] = __builtin_bit_cast(u32x4, v);
+    for (int e = 0; e < 8; ++e) {
+      high[e] = static_cast<__bf16>(x[e]);
+      low[e] = static_cast<__bf16>(x[e] - static_cast<float>(high[e]));
+    }
+    b[0] = __builtin_bit_cast(u32x4, high);
+    b[1] = __builtin_bit_cast(u32x4, low);
   }
 }
 
 // D features (64, 128 or 256, at least the width) and storage T of query and output.
 template <class T, int D>
 struct Tile {
-  static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
+  static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;       // of a query feature
+  static constexpr int kShares = sizeof(T) == 4 ? 3 : 2;      // of a softmax weight
   static constexpr int kSteps = D / 32;                       // products of a key tile
   static constexpr int kKeyWords = D / 32;                    // code words of a lane's D / 4 features
   static constexpr int kKeyScales = D == 256 ? 2 : 1;
@@ -189,7 +195,7 @@ __device__ __forceinline__ uint8_t* step_room() {
 template <class T, int D, bool kPieces, bool kWords, int QT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) void k_attend(const Args a) {
   using S = Tile<T, D>;
-  constexpr int C = S::C, kParts = S::kParts;
+  constexpr int C = S::C, kParts = S::kParts, kShares = S::kShares;
   __shared__ float2 stats[kWaves][16];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t i16 = lane % 16, g = lane / 16;
@@ -337,7 +343,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
       }
     }
 
-    u32x4 shares[QT][kParts];
+    u32x4 shares[QT][kShares];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       auto hide = [&](f32x4 (&v)[2], float value) {
@@ -377,7 +383,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
         s = weigh();
       }
       sum[t] = sum[t] + s;
-      share_operands<kParts>(e, shares[t]);
+      share_operands<kShares>(e, shares[t]);
     }
 
     if (rare(masked)) {
@@ -425,7 +431,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
       for (int w = 0; w < 4; ++w)
         v[w] = __builtin_amdgcn_perm(values[2 * w + 1][j / 2], values[2 * w][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-      for (int i = 0; i < kParts; ++i)
+      for (int i = 0; i < kShares; ++i)
 #pragma unroll
         for (int t = 0; t < QT; ++t) o[t][j] = product(v, shares[t][i], o[t][j]);
     }
