@@ -458,6 +458,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
       turn(std::integral_constant<int, 2>{}, step + 2 * kWaves);
     }
   }
+  // The loads past the last step may be under way, to rooms that the join writes.
+  __builtin_amdgcn_s_waitcnt(lds_wait(0));
+  asm volatile("" ::: "memory");
 #pragma unroll
   for (int t = 0; t < QT; ++t) sum[t] = group_sum(sum[t]);
 
