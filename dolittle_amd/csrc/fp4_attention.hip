@@ -618,7 +618,6 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks, b
   constexpr const char* kRows = "too many query rows";
   a.seq_rows = static_cast<uint32_t>(times(a.rows, a.group, 1u << 30, kRows));
   a.all_rows = static_cast<uint32_t>(times(a.seq_rows, a.batch, 1u << 30, kRows));
-  times(a.all_rows, a.kv_heads, 1u << 23, kRows);  // workgroups of the join
   // Two tiles a wavefront convert the keys and values once for both.  BF16, 512 rows of
   // 32 heads over 4096 keys: 62 us, one tile 89; 1000 rows of them, 511 keys in sight each:
   // 44 and 56; 64 rows a KV head, 4 sequences: 23 and 22.  FP32, with three products for
@@ -630,10 +629,14 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks, b
   uint64_t keys = a.capacity;
   if (a.window) keys = std::min<uint64_t>(keys, uint64_t{a.window} + a.sinks + a.tile_rows + 3 * kKeys);
   const uint64_t rounds = ceil_div(keys, kKeys * kWaves);
-  const uint64_t tasks = times(times(a.batch, a.kv_heads, kMostBlocks, "too many workgroups"), a.tiles, kMostBlocks, "too many workgroups");
-  a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(ceil_div(rounds, 2), std::max(ceil_div(512, tasks), keys / kMostRange))));
-  const uint64_t groups = times(uint64_t{a.batch} * a.kv_heads, a.splits, kMostBlocks, "too many workgroups");
-  l.blocks = static_cast<uint32_t>(times(ceil_div(groups, 8) * 8, a.tiles, kMostBlocks, "too many workgroups"));
+  constexpr const char* kTiles = "too many row tiles";
+  const uint64_t heads = times(a.batch, a.kv_heads, kMostBlocks, kTiles), tasks = times(heads, a.tiles, kMostBlocks, kTiles);
+  times(ceil_div(heads, 8) * 8, a.tiles, kMostBlocks, kTiles);
+  const uint64_t most = std::max<uint64_t>(1, kMostBlocks / a.tiles / 8 * 8 / heads);  // ranges that a launch has room for
+  a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min({ceil_div(rounds, 2), std::max(ceil_div(512, tasks), keys / kMostRange), most})));
+  // More rows than the join has workgroups for fill the card without ranges.
+  if (uint64_t{a.all_rows} * a.kv_heads > kMostBlocks) a.splits = 1;
+  l.blocks = static_cast<uint32_t>(ceil_div(heads * a.splits, 8) * 8 * a.tiles);
   if (a.splits > 1) {
     const uint64_t entries = uint64_t{a.splits} * a.kv_heads * a.all_rows;
     l.part_bytes = ceil_div(entries * 8, 256) * 256;

@@ -348,10 +348,12 @@ int dl_cache_append_fp4(dl_queue* queue, int dtype, const dl_batch_shape* shape,
  * i and sees slots j <= p; with a window (not 0) only those with j > p - window,
  * and the first `sinks` slots up to p.  Rows out of sight are not read: a step costs
  * by its window.  A row that sees no key is zeros; a key that a row does not see
- * has no effect on it, NaN groups included.  Widths up to 256.  `scale` is a device
- * word, as dl_attention's.  BF16 storage rounds every softmax weight to 2^-16 of it
- * for its product with V.  The workspace (16-byte aligned; of no bytes it may be null)
- * belongs to one call at a time; its contents need not survive. */
+ * has no effect on it, NaN groups included.  Widths up to 256; batch * kv_heads,
+ * rounded up to eights, times ceil(rows * query_heads / kv_heads / 16) is at most
+ * 2^23 - 8.  `scale` is a device word, as dl_attention's.  BF16 storage rounds every
+ * softmax weight to 2^-16 of it for its product with V.  The workspace (16-byte
+ * aligned; of no bytes it may be null) belongs to one call at a time; its contents
+ * need not survive. */
 int dl_attention_fp4_bytes(const dl_batch_shape* shape, uint64_t window, uint64_t sinks, uint64_t* bytes);
 int dl_attention_fp4(dl_queue* queue, int dtype, const dl_batch_shape* shape, const void* query,
                      const dl_fp4_cache* cache, const uint64_t* lengths, uint64_t window, uint64_t sinks, void* output,
