@@ -129,6 +129,7 @@ void k_project_staged(const ProjectArgs a, uint32_t per_group) {
   constexpr int kRoom = kStageSums + kSums * W * 1024;
   constexpr bool kSplit = sizeof(T) == 4;
   constexpr int kParts = kSplit ? 3 : 1;
+  static_assert(!(kSplit && kPieces), "FP32 rows have no form in pieces");
   static_assert(kBlocks == 1 || kRow == 128, "longer rows are cut into blocks");
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t i16 = lane % 16, g = lane / 16;
@@ -143,7 +144,7 @@ void k_project_staged(const ProjectArgs a, uint32_t per_group) {
   constexpr uint32_t kTileStep = kRow == 128 ? 0 : M / 2;
 
   u32x4 in[kBlocks][kChunks][2][4];
-  if constexpr (kSplit || !kPieces) {
+  if constexpr (!kPieces) {
     // Element by element through LDS of the wavefront's own, in the stage loaded last.
     constexpr int kHalf = 128;
     uint16_t* parts = reinterpret_cast<uint16_t*>(project_stage<kStages - 1, kRoom>()) + wave * (kParts * kRows * kHalf);
@@ -637,10 +638,12 @@ void launch_project(hipStream_t s, const ProjectArgs& a) {
     constexpr int kRow = decltype(row)::value, kBlocks = decltype(blocks)::value;
     const uint64_t sets = ceil_div(a.out_w, 2048 / kRow), per_group = ceil_div(sets, 256);
     const dim3 grid(static_cast<unsigned>(ceil_div(sets, per_group)), static_cast<unsigned>(row_tiles));
+    // FP32 rows go element by element, whole pieces or not.
+    constexpr bool kDirect = kPieces && sizeof(T) == 2;
     if (words)
-      k_project_staged<T, kPieces, true, kRow, kBlocks><<<grid, kProjectWaves * 64, 0, s>>>(a, static_cast<uint32_t>(per_group));
+      k_project_staged<T, kDirect, true, kRow, kBlocks><<<grid, kProjectWaves * 64, 0, s>>>(a, static_cast<uint32_t>(per_group));
     else
-      k_project_staged<T, kPieces, false, kRow, kBlocks><<<grid, kProjectWaves * 64, 0, s>>>(a, static_cast<uint32_t>(per_group));
+      k_project_staged<T, kDirect, false, kRow, kBlocks><<<grid, kProjectWaves * 64, 0, s>>>(a, static_cast<uint32_t>(per_group));
   };
   if (a.groups <= 32)
     run(I(32), I(1));
