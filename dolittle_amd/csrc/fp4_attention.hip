@@ -56,6 +56,10 @@ struct Args {
 
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ float reference_of(float m) { return m == -INFINITY ? 0.0f : m; }
+// The square root of 2^v, to multiply by twice: what is counted from an old maximum may
+// be kMostSum times as large, so a factor below 2^-126, which exp2 gives as zero, can
+// leave a value that is not.
+__device__ __forceinline__ float root_exp2_of(float v) { return exp2_of(0.5f * v); }
 __device__ __forceinline__ bool rare(bool condition) { return __builtin_expect(condition, false); }
 __device__ __forceinline__ float group_max(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -373,13 +377,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
 #pragma unroll
         for (int u = 0; u < 2; ++u) high = fmaxf(high, fmaxf(fmaxf(p[t][u][0], p[t][u][1]), fmaxf(p[t][u][2], p[t][u][3])));
         const float highest = group_max(high) * factor, raised = rises ? fmaxf(top[t], highest) : top[t];
-        const float less = top[t] == -INFINITY ? 1.0f : exp2_of(top[t] - raised);
+        const float less = top[t] == -INFINITY ? 1.0f : root_exp2_of(top[t] - raised);
         top[t] = raised;
         from[t] = -reference_of(raised);
         most_sum[t] = raised == -INFINITY ? -1.0f : kMostSum;
-        sum[t] = sum[t] * less;
+        sum[t] = sum[t] * less * less;
 #pragma unroll
-        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * less;
+        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * less * less;
         s = weigh();
       }
       sum[t] = sum[t] + s;
@@ -481,11 +485,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
       if (wave < half) {
         const float2 other = stats[wave + half][i16];
         const float raised = fmaxf(top[t], other.x), base = reference_of(raised);
-        const float mine = exp2_of(top[t] - base), theirs = exp2_of(other.x - base);
+        const float mine = root_exp2_of(top[t] - base), theirs = root_exp2_of(other.x - base);
         top[t] = raised;
-        sum[t] = fma_rn(sum[t], mine, other.y * theirs);
+        sum[t] = fma_rn(sum[t] * mine, mine, other.y * theirs * theirs);
 #pragma unroll
-        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * mine + room[wave][j][lane] * theirs;
+        for (int j = 0; j < C; ++j) o[t][j] = o[t][j] * mine * mine + room[wave][j][lane] * theirs * theirs;
       }
     }
   }
@@ -547,18 +551,19 @@ __global__ __launch_bounds__(kThreads) void k_join(const Args a) {
   float top = mine.x;
   for (uint32_t r = lane + 64; r < ranges; r += 64) top = fmaxf(top, part(r).x);
   const float from = reference_of(wave_max(top));
-  float sum = exp2_of(mine.x - from) * mine.y;
+  float root = root_exp2_of(mine.x - from), sum = root * mine.y * root;
   for (uint32_t r = lane + 64; r < ranges; r += 64) {
     const float2 p = part(r);
-    sum = fma_rn(exp2_of(p.x - from), p.y, sum);
+    root = root_exp2_of(p.x - from);
+    sum = fma_rn(root, root * p.y, sum);
   }
 #pragma unroll
   for (int off = 32; off; off /= 2) sum = sum + __shfl_xor(sum, off);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   auto add = [&](uint32_t r, const f32x4& v) {
-    const float share = exp2_of(part(r).x - from);
+    const float share = root_exp2_of(part(r).x - from);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = fma_rn(share, v[e], acc[e]);
+    for (int e = 0; e < 4; ++e) acc[e] = fma_rn(share, share * v[e], acc[e]);
   };
 #pragma unroll
   for (uint32_t m = 0; m < kAhead; ++m)

@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 
 import fp4_reference as ref
+from dolittle_amd.fp4 import attention_workspace_bytes
 from test_gpu_fp4 import Problem, close, value_of
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +51,26 @@ def test_attention_of_cancelling_values(oracle, device, queue, dtype, heads, row
 def test_attention_of_cancelling_values_over_ranges(oracle, device, queue, dtype):
     p = paired(oracle, dtype, 2, 1, 4000, (4, 1, 128), [4000, 1030])
     close(value_of(p.run(device, queue)), *want(p))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("batch,heads,n,second,largest", [
+    (1, 1, 300, 170, 10),    # joined with another wavefront's
+    (1, 1, 300, 170, 290),   # with another range's
+    (8, 64, 420, 170, 300),  # raised in the same wavefront
+])
+def test_a_weight_far_below_the_largest(oracle, device, queue, dtype, batch, heads, n, second, largest):
+    """The largest score is 88 and its value 0; that of the second, 8.25, is 1, so the output is exp(-79.75).  All other
+    scores are 0: the second key is counted from their maximum, which lies e^-88 below the largest, under 2^-126."""
+    p = Problem(oracle, dtype, batch, 1, n, (heads, heads, 32), [n] * batch)
+    p.kc[:], p.vc[:], p.ks[:], p.vs[:] = 0, 0, 127, 127
+    p.kc[:, :, second, 0, 0], p.kc[:, :, largest, 0, 0] = 7, 6  # 6 and 4
+    p.ks[:, :, largest] = 131
+    p.vc[:, :, second] = 0x22
+    p.q[:] = 0
+    p.q[..., 0] = 0x3fb0 if dtype == "bf16" else 1.375
+    p.scale = np.float32(1)
+    assert (attention_workspace_bytes(p.shape) == 0) == (heads == 64)
+    out, bound = want(p)
+    assert np.allclose(out, np.exp(-79.75), rtol=1e-6) and bound.max() < 0.1 * out.min()
+    close(value_of(p.run(device, queue)), out, bound)
