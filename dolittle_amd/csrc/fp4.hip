@@ -370,12 +370,12 @@ void k_project_staged(const ProjectArgs a, uint32_t per_group) {
 }
 
 // Few rows with more inputs than the staged kernel holds in registers: a workgroup per
-// 16 outputs, inputs and codes read as they are needed, four groups at once.  1 row of
-// 12,320 inputs to 4096 outputs takes 19 us (26 a group at once), where the staged
-// kernel takes 9.4 for 12,288.
+// 16 outputs, inputs and codes read as they are needed, a group's all at once.  1 row of
+// 12,320 inputs to 4096 outputs takes 16 us, where the staged kernel takes 9.4 for
+// 12,288; of 17,408 24 us.  The codes of four groups at once: 19 and 29.
 template <class T, bool kPieces>
 __global__ __launch_bounds__(kProjectWaves * 64) void k_project_long(const ProjectArgs a) {
-  constexpr int W = kProjectWaves, kRows = columns_of<T>, kParts = sizeof(T) == 4 ? 3 : 1, kAhead = 4;
+  constexpr int W = kProjectWaves, kRows = columns_of<T>, kParts = sizeof(T) == 4 ? 3 : 1;
   __shared__ f32x4 sums[W][64];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t i16 = lane % 16, g = lane / 16;
@@ -384,25 +384,17 @@ __global__ __launch_bounds__(kProjectWaves * 64) void k_project_long(const Proje
   const T* x = static_cast<const T*>(a.x) + static_cast<uint64_t>(first_row + column % rows) * a.in_w;
   const uint64_t o0 = static_cast<uint64_t>(blockIdx.x) * 16, output = min(o0 + i16, a.out_w - 1) * a.groups;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint32_t group0 = wave * 4; group0 < a.groups; group0 += 4 * W * kAhead) {
-    u32x4 code[kAhead];
-    uint32_t by[kAhead];
+  for (uint32_t group0 = wave * 4; group0 < a.groups; group0 += 4 * W) {
+    const uint32_t group = group0 + g, at = min(group, a.groups - 1);  // past the last: its inputs are zeros
+    const u32x4 code = load_stream(reinterpret_cast<const u32x4*>(a.codes) + output + at);
+    const float by = scale_of(a.scales[output + at]);
+    float v[4][8];
 #pragma unroll
-    for (int t = 0; t < kAhead; ++t) {
-      const uint32_t at = min(group0 + 4 * W * t + g, a.groups - 1);  // past the last: its inputs are zeros
-      code[t] = load_stream(reinterpret_cast<const u32x4*>(a.codes) + output + at);
-      by[t] = a.scales[output + at];
-    }
+    for (int s = 0; s < 4; ++s) load_eight<T, kPieces>(x, group * kGroup + 8 * s, a.in_w, v[s]);
 #pragma unroll
-    for (int t = 0; t < kAhead; ++t) {
-      float v[4][8];
-#pragma unroll
-      for (int s = 0; s < 4; ++s) load_eight<T, kPieces>(x, (group0 + 4 * W * t + g) * kGroup + 8 * s, a.in_w, v[s]);
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const Parts p = split(v[s]);
-        acc = product(to_bf16(code[t][s], scale_of(by[t])), kParts == 1 || part == 0 ? p.part[0] : part == 1 ? p.part[1] : p.part[2], acc);
-      }
+    for (int s = 0; s < 4; ++s) {
+      const Parts p = split(v[s]);
+      acc = product(to_bf16(code[s], by), kParts == 1 || part == 0 ? p.part[0] : part == 1 ? p.part[1] : p.part[2], acc);
     }
   }
   sums[wave][lane] = acc;
