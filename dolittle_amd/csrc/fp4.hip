@@ -94,17 +94,20 @@ template <class T>
 constexpr int columns_of = sizeof(T) == 4 ? 5 : 16;  // rows of a workgroup
 
 // The stream goes through LDS, so that every load of a wavefront is 1 KiB of one or two
-// rows: read as operands, 16 rows at a time, it came at 4 TB/s with the scales and at
-// 5.4 without, this way at 6.7 (8 rows, 4096 to 151,936, launch and end included: 66 us,
-// 5.0 TB/s; 1 row, 4096 to 1024: 3.8 us; 3 rows FP32, 12,288 to 4095: 16 us).  A stage is
+// rows: a plain read of codes and scales in the operands' order, 16 rows at a time, comes
+// at 4.1 TB/s, in their own at 6.7.  8 rows, 4096 to 151,936: 66 us, 5.0 TB/s, launch and
+// end included; 1 row, 4096 to 1024: 3.8 us; 3 rows FP32, 12,288 to 4095: 16 us.  A stage is
 // 2048 groups: kRow of 2048 / kRow outputs, M tiles of 16, loaded straight to LDS by
 // all wavefronts, kStages - 1 ahead.  Of its sixteen units of 16 outputs and 256
 // inputs a wavefront takes two.  A barrier a stage says that the stage has landed,
 // that the one before it is read and that its sums are there.  Pieces of a row lie at
 // piece ^ row, so that the 16 rows of an operand lie in distinct banks.
-// A stage's room holds its codes, its scales and the wavefronts' sums.  Objects apart,
-// and none read after loads to it were issued, so that the compiler sees no use of
-// loads in flight and waits for none.
+// A stage's room holds its codes, its scales and the wavefronts' sums.  Objects apart, so
+// that the compiler sees no use of loads in flight in a read of another stage and waits
+// for none.  That holds for BF16 rows in whole pieces.  Rows that come element by element
+// pass through the last room first, after which it waits for all loads before the first
+// read of every third stage.  Their kernels of three blocks spill too: 4 or 9 registers
+// (FP32), 24 or 26 (BF16), each read back with a wait for all loads.
 constexpr int kStageScales = 2048 * kGroupBytes, kStageSums = kStageScales + 2048;
 template <int kStage, int kBytes>
 __device__ __forceinline__ uint8_t* project_stage() {
@@ -319,8 +322,8 @@ void k_project_staged(const ProjectArgs a, uint32_t per_group) {
     if (stage && stage % kBlocks == 0) finish(room, stage / kBlocks - 1);
   };
   // A stage with two more behind it: it has landed when only the next one's loads are
-  // under way.  No load here lies under a condition: the compiler would wait for all of
-  // them before every read.
+  // under way; waits that the compiler adds make this one stricter.  No load here lies
+  // under a condition: the compiler would wait for all of them before every read.
   auto turn = [&](auto slot, uint32_t stage) __attribute__((always_inline)) {
     constexpr int kSlot = decltype(slot)::value, kBefore = (kSlot + kStages - 1) % kStages;
     __builtin_amdgcn_s_waitcnt(lds_wait((kStages - 2) * kLoads));
@@ -423,9 +426,12 @@ __device__ const u32x4 zero_piece = {0, 0, 0, 0};
 // Many rows: four wavefronts share 32 kRowTiles rows, 128 inputs at a time through
 // LDS, loaded kStages - 1 steps ahead; each has 32 outputs of its own, whose codes come
 // straight from memory as far ahead, so that every code is converted once for all the
-// rows.  32 x 32 products: 2440 TFLOP/s against 1460 of 16 x 16 ones.  512 rows, 4096
-// to 6144: 37 us, 690 TFLOP/s; bound by the conversions beside the products and 1.5
-// tiles a compute unit.
+// rows.  A 32 x 32 product does twice the operations of a 16 x 16 one for the operands it
+// reads; the rates are the same.  512 rows, 4096 to 6144: 39 us, 660 TFLOP/s, 45 with
+// weights that no call has read lately.  Products are busy 24% of that, vector instructions
+// issue in 19%, and wavefronts wait to issue 47%: the 384 tiles run at once, one or two a
+// compute unit, so one or two wavefronts a SIMD cover few of each other's waits and half of
+// the units end early.
 template <int kStage, int kBytes>
 __device__ __forceinline__ uint8_t* many_stage() {
   __shared__ __align__(1024) uint8_t room[kBytes];
@@ -599,8 +605,9 @@ void launch_project(hipStream_t s, const ProjectArgs& a) {
   const bool words = a.groups % 4 == 0 && reinterpret_cast<uintptr_t>(a.scales) % 4 == 0;
   // Few rows read the weights once per 16 (FP32 5); many convert them once per 32 or 64
   // and need tiles for most compute units.  4096 x 4096, rows 24, 48 and 128: few 11, 18
-  // and 45 us, many by 32 rows 17, 17 and 18, by 64 19, 20 and 20; 4096 x 24576, 48 and
-  // 128 rows: few 40 and 97, by 32 42 and 61, by 64 29 and 51.
+  // and 44 us, many by 32 rows 17, 17 and 18, by 64 19, 20 and 21; 4096 x 24576, 48 and
+  // 128 rows: few 41 and 97, by 32 42 and 62, by 64 29 and 51.  FP32, 4096 x 4096, rows 20
+  // and 24: few 26 and 32, many 37 and 37.
   if (a.rows > (sizeof(T) == 4 ? 20 : 32)) {
     auto many = [&](auto whole_words, auto tiles) {
       constexpr int kRowTiles = decltype(tiles)::value;
@@ -686,8 +693,9 @@ __device__ __forceinline__ f32x4 load_four(const T* from) {
 // rounding.  32 lanes take a head, eight features each, and four of them a group.
 // What bounds it for few rows is one wait for memory and the 64-bit angles, so the
 // rows are asked for before the angles are computed: 8 rows of 32 and 8 heads of 128
-// features 6.2 us, 1 us less than without that; 1024 FP32 rows 13, 3.4 less.  kFours: halves are of
-// whole fours, all rows at their alignment.
+// features 5.6 us, 1024 FP32 rows 11.5 (wavefronts wait for memory or a barrier half the
+// time), BF16 9.0.  kFours: halves are of whole fours, all rows at their alignment; feature
+// by feature these take 7.3, 19 and 15.
 template <class T, bool kFours>
 __global__ __launch_bounds__(kAppendThreads) void k_append(const AppendArgs a, bool advance_here) {
   __shared__ __align__(16) float cosine[kMostWidth / 2], sine[kMostWidth / 2];

@@ -13,8 +13,9 @@
 // their own, two steps ahead.  Ranges leave their maximum, sum and unnormalised
 // output, which k_join joins; a single range writes the output itself.  Of few rows the
 // caches' stream is the bound: 64 sequences of up to 32,768 keys, 8 KV heads of 128
-// features, 292 us, 5.2 TB/s; of many the conversions and exponentials beside the
-// products: 512 rows of 32 heads over 4096 keys 59 us, 540 TFLOP/s, FP32 123.
+// features, 300 us, 5.0 TB/s; of many the conversions and exponentials beside the
+// products: 512 rows of 32 heads over 4096 keys 73 us, 440 TFLOP/s, FP32 126.  There vector
+// instructions issue in half of the cycles and products are busy in 27%.
 //
 // Operands.  A lane takes D / 4 neighbouring features of a key's codes, one to two
 // groups or half of one, and converts them to the first operands of the products K
@@ -195,7 +196,8 @@ __device__ __forceinline__ uint8_t* step_room() {
 }
 
 // Of two tiles of rows a wavefront holds twice the queries and outputs: left to itself
-// the compiler takes 300 registers, one workgroup a unit, 91 us where this takes 62.
+// the compiler takes more than 256 registers, one workgroup a unit, 102 us where this
+// takes 73.
 template <class T, int D, bool kPieces, bool kWords, int QT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) void k_attend(const Args a) {
   using S = Tile<T, D>;
@@ -241,7 +243,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QT))) 
   // query has zeros there, and such features of the output are not stored.  Piece p of a
   // key's codes lies at p ^ key / 8, so that the keys of an operand lie in distinct banks.
   // Whole rows of scale words go through LDS too, 1 load (D = 256: 2) for 10 (12): 512 rows
-  // over 4096 keys 59.5 us for 61.6, 8 sequences of 4607 keys 18.0 for 18.5.
+  // over 4096 keys 75 us for 77, 64 sequences of up to 32,768 keys 318 for 330.
   constexpr uint32_t P = D / 32, kRowBytes = D / 2, kHalf = 16 * D;  // pieces of a key; bytes of 32
   constexpr uint32_t kRoom = 2 * kHalf + (kWords ? 2 * D : 0), kWordRow = kWords ? D / 128 : 1;
   const uint32_t value_group = min(i16 * C / kGroup, a.groups - 1);
@@ -624,9 +626,10 @@ Layout layout_of(const dl_batch_shape* shape, uint64_t window, uint64_t sinks, b
   a.seq_rows = static_cast<uint32_t>(times(a.rows, a.group, 1u << 30, kRows));
   a.all_rows = static_cast<uint32_t>(times(a.seq_rows, a.batch, 1u << 30, kRows));
   // Two tiles a wavefront convert the keys and values once for both.  BF16, 512 rows of
-  // 32 heads over 4096 keys: 62 us, one tile 89; 1000 rows of them, 511 keys in sight each:
-  // 44 and 56; 64 rows a KV head, 4 sequences: 23 and 22.  FP32, with three products for
-  // one: 140 and 129.  Of 256 features two tiles do not fit the registers.
+  // 32 heads over 4096 keys: 75 us, one tile 100; 1000 rows of them, 511 keys in sight each:
+  // 47 and 59; 64 rows a KV head, 4 sequences: 25 and 23.  FP32, with three products for
+  // one, gains less: 512 rows 116 and 126, 64 rows of 4 sequences 67 and 61, 100 rows over 2000
+  // keys 35 and 32; it stays with one.  Of 256 features two tiles do not fit the registers.
   a.tile_rows = bf16 && a.width <= 128 && a.seq_rows > 64 ? 32 : 16;
   a.tiles = static_cast<uint32_t>(ceil_div(a.seq_rows, a.tile_rows));
   a.pitch = (a.width + 3) / 4 * 4;

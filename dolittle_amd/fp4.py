@@ -12,7 +12,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from .batch import _BYTES, _CODES, BatchShape, _at
+from .batch import _CODES, BatchShape, _at
 from .runtime import Device, DeviceBuffer, Queue
 
 CacheAddresses = _lib.Fp4Cache
@@ -65,7 +65,8 @@ class Fp4Weight:
 
 class Fp4Cache:
     """The caches of `batch` sequences in 4 bits, read whole or through a sliding
-    window with first rows that stay visible.
+    window with first rows that stay visible.  A window bounds what a step reads and not
+    what the cache holds: `capacity` is for every row of a sequence.
 
     The host keeps each sequence's length, so a row that does not fit is refused
     here.  Every method only enqueues, except that a first attend that needs more

@@ -331,14 +331,17 @@ int dl_fp4_values(dl_queue* queue, int dtype, const void* codes, const void* sca
                   uint64_t width);
 /* dl_projection with 4-bit weights: Y[R,O] = X[R,I] W[O,I]^T, one rounding of the
  * FP32 sum.  Up to 32 rows (FP32 20) read the weights once per 16 (5) of them, more
- * convert them once per 32 or 64; a NaN group makes its output NaN. */
+ * convert them once per 32 or 64; a NaN group makes its output NaN.  Rows and outputs up
+ * to 2^30; of more than 32 (20) rows at most 2^23 tiles of 64 (32) rows by 128 outputs,
+ * outputs rounded up to 1024; else, of more than 12,288 inputs, at most 2^26 outputs. */
 int dl_projection_fp4(dl_queue* queue, int dtype, const void* input, const void* codes, const void* scales,
                       void* output, uint64_t rows, uint64_t input_width, uint64_t output_width,
                       const uint64_t* output_position);
 /* dl_cache_append to a cache held in 4 bits (no slots and weights: nothing is
  * evicted from it).  Rotated keys go from FP32 to 4 bits in one rounding.  Rows
- * past the capacity are dropped, the length stays at the capacity.  Head widths up
- * to 256, even.  query_out may be query, lengths_out and positions_out their
+ * past the capacity are dropped, the length stays at the capacity: the cache holds
+ * every row of a sequence, under a window too.  Head widths up to 256, even; up to
+ * 65,535 sequences.  query_out may be query, lengths_out and positions_out their
  * inputs. */
 int dl_cache_append_fp4(dl_queue* queue, int dtype, const dl_batch_shape* shape, const void* query, const void* key,
                         const void* value, void* query_out, const dl_fp4_cache* cache, const uint64_t* lengths,
@@ -346,9 +349,11 @@ int dl_cache_append_fp4(dl_queue* queue, int dtype, const dl_batch_shape* shape,
 /* out = softmax(scale * Q K^T) V over each sequence's cache.  `lengths` includes
  * the new rows, which are the last `rows`: new row i is at slot p = length - rows +
  * i and sees slots j <= p; with a window (not 0) only those with j > p - window,
- * and the first `sinks` slots up to p.  Rows out of sight are not read: a step costs
- * by its window.  A row that sees no key is zeros; a key that a row does not see
- * has no effect on it, NaN groups included.  Widths up to 256; batch * kv_heads,
+ * and the first `sinks` slots up to p.  A step costs by its window.  Slots below the
+ * length that a row does not see may be read where they share a step of 32 slots or a
+ * tile of new rows with ones that are seen, so they are readable memory; slots from the
+ * length on are not read.  A row that sees no key is zeros; a key that a row does not
+ * see has no effect on it, NaN groups included.  Widths up to 256; batch * kv_heads,
  * rounded up to eights, times ceil(rows * query_heads / kv_heads / 16) is at most
  * 2^23 - 8.  `scale` is a device word, as dl_attention's.  BF16 storage rounds every
  * softmax weight to 2^-16 of it for its product with V.  The workspace (16-byte
